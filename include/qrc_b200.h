@@ -275,6 +275,135 @@ int qrc_free_like(qrc_vmm_buf* buf);
  * d_x == d_y does nothing.  Asynchronous.  No reference counterpart. */
 int qrc_copy_f32(const float* d_x, float* d_y, size_t n, qrc_ctx* ctx, void* stream);
 
+/* Element types of the entry points that take more than one. */
+enum qrc_type { QRC_F32 = 0, QRC_BF16 = 1, QRC_F16 = 2 };
+
+/* --- One norm over many tensors (a training step's gradients) ---------------
+ *
+ * A list is a plan over tensors that the caller owns: it keeps their
+ * addresses and sizes on the host, holds no device memory and never changes,
+ * so any number of threads, streams and captured graphs may use one list at
+ * the same time, each call with a workspace of its own.  A captured call
+ * carries a copy of the plan: the list may be destroyed afterwards, the
+ * tensors have to stay.
+ *
+ * A tensor is `rows` rows of `cols` neighbouring elements.  Row r of the
+ * input starts at d_in + r * in_pitch elements, of the output at
+ * d_out + r * out_pitch; a dense tensor of n elements is rows = 1, cols = n
+ * (the pitches are then not read).  d_in and d_out need the alignment of their
+ * types only.  d_out == NULL: the list serves norms alone (out_type is not
+ * read).  d_out == d_in with the same type and pitch: scaled in place.
+ * Tensors without elements are allowed. */
+typedef struct qrc_tensor {
+    const void* d_in;
+    void* d_out;
+    uint64_t rows, cols;
+    uint64_t in_pitch, out_pitch;   /* elements; below 2^32 */
+    int32_t in_type, out_type;      /* qrc_type */
+} qrc_tensor;
+
+typedef struct qrc_list qrc_list;
+
+enum qrc_norm {
+    QRC_NORM_INF = 0,               /* max |x| */
+    QRC_NORM_1 = 1,                 /* sum |x| */
+    QRC_NORM_2 = 2                  /* sqrt(sum x^2) */
+};
+
+/* Makes a list for `device`.  At most 2^40 elements (QRC_ERR_RANGE).  No GPU
+ * work.  No counterpart in the reference, nor for the functions below. */
+int qrc_list_create(qrc_list** out, int device, const qrc_tensor* tensors, size_t count);
+int qrc_list_destroy(qrc_list* list);
+
+/* 1 when qrc_list_clip may write these tensors' outputs: every tensor has one
+ * and no output shares memory with another output, nor with an input other
+ * than its own in the same place (the same tensor twice in place, for
+ * instance, would be scaled twice).  0 when not, or when it cannot be shown;
+ * a negative qrc_status for tensors that qrc_list_create refuses.  Runs on
+ * the host. */
+int qrc_list_writable(const qrc_tensor* tensors, size_t count);
+
+/* Bytes of device workspace (8-byte aligned) that a call on the list needs.
+ * Its contents do not matter, before or after. */
+size_t qrc_list_workspace(const qrc_list* list);
+
+/* *d_norm = the norm (qrc_norm) over all elements of all tensors.  Sums are
+ * accumulated in double (16-bit inputs eight terms at a time in float first)
+ * in an order that depends on the list alone, so a repeated call gives the
+ * same bits.  A NaN element gives NaN, unlike in qrc_absmax_f32; an empty
+ * list gives 0.  Asynchronous on `stream`. */
+int qrc_list_norm(const qrc_list* list, int norm, float* d_norm, void* d_work, void* stream);
+
+/* Scales every tensor into its output by
+ *   k = min(1, max_norm / (norm + 1e-6))
+ * (k in double, rounded to float; the product in float, rounded to the
+ * output's type).  The norm is computed first and written to *d_norm (which
+ * may be NULL); or, with d_given, is the float at d_given, such as the norm
+ * over several GPUs, and d_norm and d_work are not used.  A NaN norm makes
+ * the outputs NaN; max_norm infinite gives k = 1.  With k = 1 tensors in
+ * place are left as they are.  QRC_ERR_INVALID when the list is not writable
+ * (qrc_list_writable) or max_norm is negative or NaN.  Asynchronous. */
+int qrc_list_clip(const qrc_list* list, int norm, double max_norm, const float* d_given, float* d_norm,
+                  void* d_work, void* stream);
+
+/* --- Weights in 4 bits with a scale per group of columns --------------------
+ *
+ *   value[n][k] = (code[n][k] - zero[g][n]) * scale[g][n],   g = k / group
+ *
+ * d_packed holds n rows of ceil(k / 128) blocks of 16 words (16-byte
+ * aligned).  Word 4*t + j of a block (t, j < 4) holds columns
+ * 32*j + 8*t + 0..7 of the block's 128: column 2*i in bits 4*i..4*i+3, column
+ * 2*i + 1 in bits 16 + 4*i..19 + 4*i.  Codes behind column k may be anything.
+ * d_scales is [ceil(k / group)][n] of `type`; d_zeros is [ceil(k / group)][n]
+ * whole numbers 0..15, or NULL: every zero is 8.  Rows and columns go up to
+ * 2^31.  The memory is the caller's; an output that overlaps an input is refused
+ * (QRC_ERR_INVALID). */
+typedef struct qrc_w4 {
+    uint32_t* d_packed;
+    void* d_scales;
+    uint8_t* d_zeros;
+    uint64_t n, k;
+    int32_t group;                  /* 32, 64, 128 or 256 */
+    int32_t type;                   /* QRC_BF16 or QRC_F16 */
+} qrc_w4;
+
+/* Words of d_packed for an n x k matrix. */
+uint64_t qrc_w4_words(uint64_t n, uint64_t k);
+
+/* Quantizes d_w (n rows of k elements of w->type, ld elements apart) into w's
+ * memory.  Per row and group, over the finite elements (rn: to nearest even
+ * in w->type):
+ *   symmetric:  scale = rn(max |x| / 7),  zero 8 (w->d_zeros has to be NULL)
+ *   otherwise:  scale = rn((max(x, 0) - min(x, 0)) / 15),
+ *               zero = rint(-min(x, 0) / scale), within 0..15
+ *   code = rint(x / scale) + zero, within 1..15 (symmetric) or 0..15
+ * NaN gets the code `zero` (value 0); infinities get the last code on their
+ * side; a scale of 0 gives every element the code `zero`.  Asynchronous. */
+int qrc_w4_quant(int device, const void* d_w, uint64_t ld, int symmetric, const qrc_w4* w, void* stream);
+
+/* Packs codes held one per byte (n rows of k, ld bytes apart; the low four
+ * bits count) into w->d_packed.  w's scales and zeros are not read.
+ * Asynchronous. */
+int qrc_w4_pack(int device, const uint8_t* d_codes, uint64_t ld, const qrc_w4* w, void* stream);
+
+/* d_out (n rows of k elements of out_type, ld elements apart) = the values,
+ * rounded once; values beyond out_type's range give its largest finite number.
+ * Asynchronous. */
+int qrc_w4_dequant(int device, const qrc_w4* w, void* d_out, uint64_t ld, int out_type, void* stream);
+
+/* d_y[i][j] = sum_k value[j][k] * d_x[i][k] (+ d_bias[j]) for m rows of
+ * activations (rows ldx and ldy elements apart).  d_x and d_bias (may be NULL)
+ * are of w->type, d_y of y_type: w->type or QRC_F32.  Products and sums are
+ * formed in float, per group before its scale (so |x| * 15 * group has to
+ * stay in float's range), in an order that depends on the sizes alone; the
+ * result is rounded once.  Made for a few rows (a decode step); any m >= 0
+ * works.  Rows of d_x that do not start on 16
+ * bytes need a workspace (16-byte aligned, qrc_w4_matvec_workspace bytes; 0
+ * when none is needed).  Asynchronous. */
+int qrc_w4_matvec(int device, const qrc_w4* w, const void* d_x, uint64_t m, uint64_t ldx, const void* d_bias,
+                  void* d_y, uint64_t ldy, int y_type, void* d_work, void* stream);
+size_t qrc_w4_matvec_workspace(const qrc_w4* w, const void* d_x, uint64_t m, uint64_t ldx);
+
 /* Synthetic inputs generated on the device; element i of the stream is a pure
  * function of (seed, offset + i), so shards of one stream can be generated
  * independently.  uniform[-1,1) on a 2^-23 grid; normal(0, sigma) is the

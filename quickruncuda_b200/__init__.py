@@ -7,6 +7,10 @@ Layout:
                             device code of the C-ABI library
   csrc/qrc_abi.cu           libqrc_b200.so: contexts, launches, quantize, generators
   harness/qrc_harness.cpp   C++ harness running kernel files like QuickRunCUDA
+  csrc/qrc_list.cu          one norm over many tensors and scaling them by it
+  csrc/qrc_w4.cu            4-bit weights: quantize, dequantize, product
+  tensor_list.py            gradient norm and clipping over a list of tensors
+  weight4.py                4-bit weight matrices
   api.py / _native.py       Python binding of the C ABI (ctypes)
   build.py                  in-tree nvcc build (sm_100a)
 """
@@ -16,6 +20,8 @@ from ._native import (MODE_IGNORE_PAGE_BITS, MODE_SIDE_AWARE, MODE_STREAM, MODE_
                       QrcError, load)
 from .api import (SideAwareContext, fill_normal, fill_normal_bf16, fill_uniform, host_fill_normal,
                   host_fill_uniform, outlier)
+from .tensor_list import TensorList
+from .weight4 import Weight4, quant_w4
 
 PACKAGE_DIR = Path(__file__).resolve().parent
 KERNEL_FILE = PACKAGE_DIR / "csrc" / "side_aware_b200.cu"
@@ -23,4 +29,4 @@ HARNESS = PACKAGE_DIR / "bin" / "qrc_harness"
 
 __all__ = ["SideAwareContext", "fill_uniform", "fill_normal", "fill_normal_bf16", "host_fill_uniform",
            "host_fill_normal", "outlier", "load", "QrcError", "MODE_SIDE_AWARE", "MODE_IGNORE_PAGE_BITS",
-           "MODE_WRONG_SIDE", "MODE_STREAM", "KERNEL_FILE", "HARNESS"]
+           "MODE_WRONG_SIDE", "MODE_STREAM", "KERNEL_FILE", "HARNESS", "TensorList", "Weight4", "quant_w4"]

@@ -44,6 +44,9 @@ MODE_NAMES = {"side_aware": MODE_SIDE_AWARE, "ignore_page_bits": MODE_IGNORE_PAG
               "random_side": MODE_IGNORE_PAGE_BITS, "wrong_side": MODE_WRONG_SIDE,
               "stream": MODE_STREAM}
 
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
+NORM_INF, NORM_1, NORM_2 = 0, 1, 2
+
 SIDE_OK = 0
 SIDE_NOT_RUN = 100
 
@@ -56,6 +59,18 @@ class SideInfo(ctypes.Structure):
 
     def as_dict(self) -> dict:
         return {name: getattr(self, name) for name, _ in self._fields_ if name != "reserved"}
+
+
+class Tensor(ctypes.Structure):
+    """qrc_tensor: one tensor of a list."""
+    _fields_ = [("d_in", c_void_p), ("d_out", c_void_p), ("rows", c_u64), ("cols", c_u64),
+                ("in_pitch", c_u64), ("out_pitch", c_u64), ("in_type", ctypes.c_int32), ("out_type", ctypes.c_int32)]
+
+
+class W4(ctypes.Structure):
+    """qrc_w4: a 4-bit weight matrix."""
+    _fields_ = [("d_packed", c_void_p), ("d_scales", c_void_p), ("d_zeros", c_void_p), ("n", c_u64), ("k", c_u64),
+                ("group", ctypes.c_int32), ("type", ctypes.c_int32)]
 
 
 # (name, restype, argtypes) for every entry point of the two headers.
@@ -88,6 +103,19 @@ SIGNATURES = [
     ("qrc_absmax_f32_host", c_int, [c_void_p, c_size, ctypes.POINTER(c_float), c_void_p, c_void_p]),
     ("qrc_host_reserve", c_int, [c_void_p, c_size]),
     ("qrc_amax_quant_e4m3", c_int, [c_void_p, c_size, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    ("qrc_list_create", c_int, [ctypes.POINTER(c_void_p), c_int, ctypes.POINTER(Tensor), c_size]),
+    ("qrc_list_destroy", c_int, [c_void_p]),
+    ("qrc_list_writable", c_int, [ctypes.POINTER(Tensor), c_size]),
+    ("qrc_list_workspace", c_size, [c_void_p]),
+    ("qrc_list_norm", c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
+    ("qrc_list_clip", c_int, [c_void_p, c_int, ctypes.c_double, c_void_p, c_void_p, c_void_p, c_void_p]),
+    ("qrc_w4_words", c_u64, [c_u64, c_u64]),
+    ("qrc_w4_quant", c_int, [c_int, c_void_p, c_u64, c_int, ctypes.POINTER(W4), c_void_p]),
+    ("qrc_w4_pack", c_int, [c_int, c_void_p, c_u64, ctypes.POINTER(W4), c_void_p]),
+    ("qrc_w4_dequant", c_int, [c_int, ctypes.POINTER(W4), c_void_p, c_u64, c_int, c_void_p]),
+    ("qrc_w4_matvec", c_int, [c_int, ctypes.POINTER(W4), c_void_p, c_u64, c_u64, c_void_p, c_void_p, c_u64, c_int,
+                              c_void_p, c_void_p]),
+    ("qrc_w4_matvec_workspace", c_size, [ctypes.POINTER(W4), c_void_p, c_u64, c_u64]),
     ("qrc_fill_uniform_f32", c_int, [c_void_p, c_size, c_u64, c_u64, c_void_p]),
     ("qrc_fill_normal_f32", c_int, [c_void_p, c_size, c_u64, c_u64, c_float, c_void_p]),
     ("qrc_fill_normal_bf16", c_int, [c_void_p, c_size, c_u64, c_u64, c_float, c_void_p]),

@@ -29,8 +29,10 @@ GENCODE = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_COMMON = GENCODE + ["-lineinfo", "-O3", "--std=c++17", "-Xptxas", "-v",
                          "-Xcompiler", "-fPIC,-fopenmp,-fvisibility=hidden"]
 
-LIB_SOURCES = [CSRC / "qrc_abi.cu", CSRC / "qrc_noalloc.cu", CSRC / "side_aware_b200.cu", CSRC / "qrc_gen.cuh",
+LIB_UNITS = [CSRC / "qrc_abi.cu", CSRC / "qrc_noalloc.cu", CSRC / "qrc_list.cu", CSRC / "qrc_w4.cu"]
+LIB_HEADERS = [CSRC / "side_aware_b200.cu", CSRC / "qrc_gen.cuh", CSRC / "qrc_host.h",
                INCLUDE / "qrc_b200.h", INCLUDE / "qrc_b200_debug.h"]
+LIB_SOURCES = LIB_UNITS + LIB_HEADERS
 HARNESS_SOURCES = [PKG / "harness" / "qrc_harness.cpp", CSRC / "qrc_gen.cuh"]
 
 LIB_PATH = LIB_DIR / "libqrc_b200.so"
@@ -64,8 +66,7 @@ def build_lib(checked: bool = False, force: bool = False, verbose: bool = False)
         return out
     LIB_DIR.mkdir(parents=True, exist_ok=True)
     tmp = out.with_suffix(".so.tmp")
-    cmd = [NVCC, *NVCC_COMMON, "-shared", "-o", str(tmp), str(CSRC / "qrc_abi.cu"), str(CSRC / "qrc_noalloc.cu"),
-           "-lgomp"]
+    cmd = [NVCC, *NVCC_COMMON, "--threads", "0", "-shared", "-o", str(tmp), *map(str, LIB_UNITS), "-lgomp"]
     if checked:
         cmd.insert(1, "-DQRC_CHECKED")
     _run(cmd, log=LIB_DIR / (out.name + ".buildlog"), verbose=verbose)

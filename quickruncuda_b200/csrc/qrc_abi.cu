@@ -7,6 +7,7 @@
 #define QRC_NO_PLUGIN_ABI
 #include "side_aware_b200.cu"
 #include "qrc_gen.cuh"
+#include "qrc_host.h"
 #include "../../include/qrc_b200.h"
 #include "../../include/qrc_b200_debug.h"
 
@@ -19,8 +20,6 @@
 #include <utility>
 #include <vector>
 #include <omp.h>
-
-#define QRC_API extern "C" __attribute__((visibility("default")))
 
 // ---------------------------------------------------------------------------
 // Kernels
@@ -770,32 +769,6 @@ __global__ void qrc_k_fill_normal_bf16(uint16_t* out, qrc_u64 n, qrc_u64 key, qr
 // ---------------------------------------------------------------------------
 
 namespace {
-
-thread_local int g_last_cuda = 0;
-
-#define QRC_CK(call)                                                      \
-    do {                                                                  \
-        cudaError_t e_ = (call);                                          \
-        if (e_ != cudaSuccess) { g_last_cuda = (int)e_; return QRC_ERR_CUDA; } \
-    } while (0)
-
-// Makes `dev` current for the scope and restores the caller's device.  When
-// `dev` is already current nothing is touched, so a context the caller made
-// current through the driver API (as the QuickRunCUDA harness does with
-// cuCtxCreate) stays current.
-struct DeviceScope {
-    int prev = -1;
-    bool ok = false, switched = false;
-    explicit DeviceScope(int dev) {
-        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-        if (prev == dev) { ok = true; return; }
-        ok = cudaSetDevice(dev) == cudaSuccess;
-        switched = ok && prev >= 0;
-    }
-    ~DeviceScope() { if (switched) cudaSetDevice(prev); }
-};
-
-inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 constexpr size_t kMapHeaderWords = qrc::O_PAGE_BITS;
 

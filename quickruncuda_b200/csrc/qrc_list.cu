@@ -1,0 +1,611 @@
+// qrc_list.cu -- one norm over many tensors, and scaling them by it
+// (qrc_list_*): the gradient norm and gradient clipping of a training step.
+//
+//   norm:  L1 = sum |x|, L2 = sqrt(sum x^2), Linf = max |x| over all elements
+//   clip:  y = x * k with k = min(1, max_norm / (norm + 1e-6))
+//
+// Both are bound by memory: the norm reads every byte once, the scale pass
+// reads it again and writes it.  Nothing is kept between calls: every block
+// writes its partial result to the caller's workspace, and whoever needs the
+// norm adds the partials in a fixed order, so results do not change from run
+// to run and no counter has to be zeroed.  The list of tensors travels in the
+// kernel's parameters, so a captured launch carries its own copy.
+#include "qrc_host.h"
+#include "../../include/qrc_b200.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <new>
+#include <type_traits>
+#include <vector>
+
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kMaxBlocks = 2368;              // 16 blocks per SM: what SMs differ in speed evens out
+constexpr int kMinChunkLog2 = 12, kMaxChunkLog2 = 15;
+constexpr int kKindShift = 56;                // n_kind: elements, input type << 56, output type << 60
+
+// One tensor: `n` elements at in and out.  cols == 0: dense; else rows of
+// `cols` elements that start in_pitch and out_pitch elements apart.
+struct Entry {
+    const void* in;
+    void* out;
+    uint64_t n_kind;
+    uint32_t cols, in_pitch, out_pitch;
+    uint32_t first;                           // chunks of the launch before this tensor
+};
+static_assert(sizeof(Entry) == 40, "the table has to fit in the kernel parameters");
+
+// Kernel parameters hold at most 32,764 bytes; a short list travels in the
+// small table.
+constexpr int kSmallTable = 96, kLargeTable = 812;
+
+template <int CAP>
+struct Table {
+    Entry e[CAP];
+    uint32_t count, chunks, chunk_log2, first_partial;
+};
+static_assert(sizeof(Table<kLargeTable>) + 32 <= 32764, "kernel parameter limit");
+
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+__device__ __forceinline__ uint4 load_once(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+
+template <class T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+
+template <class T> __device__ __forceinline__ void unpack(const uint4& v, float (&f)[16 / sizeof(T)]) {
+    const T* p = reinterpret_cast<const T*>(&v);
+#pragma unroll
+    for (int i = 0; i < 16 / (int)sizeof(T); i++) f[i] = to_float(p[i]);
+}
+
+// -- accumulators: sums are held in 64 bits, the maximum as the bits of |x|
+//    (a NaN's bits are above infinity's, so a NaN anywhere is the maximum) --
+
+template <int NORM>
+struct Acc {
+    double a = 0.0, b = 0.0;
+    __device__ __forceinline__ void one(float x) {
+        if (NORM == QRC_NORM_2) a = fma((double)x, (double)x, a);
+        else a += fabs((double)x);
+    }
+    template <class T> __device__ __forceinline__ void vec(const uint4& v) {
+        constexpr int VE = 16 / sizeof(T);
+        float f[VE];
+        unpack<T>(v, f);
+        if (sizeof(T) == 4) {
+            one(f[0]);
+            if (NORM == QRC_NORM_2) b = fma((double)f[1], (double)f[1], b);
+            else b += fabs((double)f[1]);
+            one(f[2]);
+            if (NORM == QRC_NORM_2) b = fma((double)f[3], (double)f[3], b);
+            else b += fabs((double)f[3]);
+            return;
+        }
+        // Eight 16-bit values: their squares are exact in float, and the sum
+        // of eight non-negative terms is off by 7 * 2^-24 of itself at most.
+        // One conversion and one add in 64 bits per 16 bytes keep the FP64
+        // pipe (16 conversions per SM and clock) off the critical path.
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < VE; i += 2) {
+            if (NORM == QRC_NORM_2) { s0 = fmaf(f[i], f[i], s0); s1 = fmaf(f[i + 1], f[i + 1], s1); }
+            else { s0 += fabsf(f[i]); s1 += fabsf(f[i + 1]); }
+        }
+        const float s = s0 + s1;
+        // fp16 squares and sums stay far inside float's range; bf16's can
+        // leave it on both sides: those eight are added one by one.
+        const bool plain = std::is_same<T, __half>::value ? true
+                           : NORM == QRC_NORM_2 ? (s >= 0x1p-90f && s <= 0x1p120f) : s <= 0x1p120f;
+        if (plain) a += (double)s;
+        else if (((v.x | v.y | v.z | v.w) & 0x7fff7fffu) != 0) {
+#pragma unroll
+            for (int i = 0; i < VE; i++) one(f[i]);
+        }
+    }
+    __device__ __forceinline__ double value() const { return a + b; }
+};
+
+template <>
+struct Acc<QRC_NORM_INF> {
+    uint32_t m = 0;
+    __device__ __forceinline__ void one(float x) { m = max(m, __float_as_uint(x) & 0x7fffffffu); }
+    template <class T> __device__ __forceinline__ void vec(const uint4& v) {
+        float f[16 / sizeof(T)];
+        unpack<T>(v, f);
+#pragma unroll
+        for (int i = 0; i < 16 / (int)sizeof(T); i++) one(f[i]);
+    }
+    __device__ __forceinline__ double value() const { return (double)__uint_as_float(m); }
+};
+
+// Combines two partial results; a NaN stays.
+template <int NORM> __device__ __forceinline__ double combine(double x, double y) {
+    if (NORM != QRC_NORM_INF) return x + y;
+    return (x > y || x != x) ? x : y;
+}
+
+// The combination of every thread's value, in a fixed order, in all threads.
+template <int NORM> __device__ __forceinline__ double block_combine(double v) {
+    __shared__ double s_part[kThreads / 32];
+    __shared__ double s_all;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v = combine<NORM>(v, __shfl_xor_sync(0xffffffffu, v, d));
+    if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double t = s_part[0];
+#pragma unroll
+        for (int i = 1; i < kThreads / 32; i++) t = combine<NORM>(t, s_part[i]);
+        s_all = t;
+    }
+    __syncthreads();
+    return s_all;
+}
+
+// -- the walk of a block's chunks ---------------------------------------------
+
+template <int CAP> __device__ __forceinline__ int find_entry(const Table<CAP>& t, uint32_t chunk) {
+    int lo = 0, hi = (int)t.count - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (t.e[mid].first <= chunk) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+// Calls fn(entry, first element, one past the last) for every tensor part of
+// block `block`'s share of the launch's chunks.
+template <int CAP, class F>
+__device__ __forceinline__ void for_share(const Table<CAP>& t, uint32_t block, uint32_t blocks, F fn) {
+    uint32_t c = (uint32_t)((uint64_t)block * t.chunks / blocks);
+    const uint32_t end = (uint32_t)((uint64_t)(block + 1) * t.chunks / blocks);
+    for (int i = find_entry(t, c); c < end; i++) {
+        const Entry& e = t.e[i];
+        const uint32_t next = i + 1 < (int)t.count ? t.e[i + 1].first : t.chunks;
+        const uint32_t stop = min(end, next);
+        const uint64_t n = e.n_kind & ((1ull << kKindShift) - 1);
+        const int shift = t.chunk_log2 - (((e.n_kind >> kKindShift) & 15) == QRC_F32 ? 2 : 1);
+        const uint64_t e0 = (uint64_t)(c - e.first) << shift;
+        const uint64_t e1 = min(n, (uint64_t)(stop - e.first) << shift);
+        fn(e, e0, e1);
+        c = stop;
+    }
+}
+
+// -- norm ----------------------------------------------------------------------
+
+template <class T, class A>
+__device__ __forceinline__ void norm_dense(const T* p, uint64_t n, A& acc) {
+    constexpr int VE = 16 / sizeof(T), U = 4;
+    const uint64_t lead = ((16 - ((uintptr_t)p & 15)) & 15) / sizeof(T);
+    const uint32_t head = (uint32_t)min(n, lead);
+    if (threadIdx.x < head) acc.one(to_float(p[threadIdx.x]));
+    p += head;
+    n -= head;
+    const uint4* v = reinterpret_cast<const uint4*>(p);
+    const uint32_t nv = (uint32_t)(n / VE);
+    uint32_t i = threadIdx.x;
+    for (; i + (U - 1) * kThreads < nv; i += U * kThreads) {
+        uint4 r[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) r[u] = load_once(v + i + u * kThreads);
+#pragma unroll
+        for (int u = 0; u < U; u++) acc.template vec<T>(r[u]);
+    }
+    for (; i < nv; i += kThreads) acc.template vec<T>(load_once(v + i));
+    const uint32_t tail = (uint32_t)(n - (uint64_t)nv * VE);
+    if (threadIdx.x < tail) acc.one(to_float(p[(uint64_t)nv * VE + threadIdx.x]));
+}
+
+template <class T, class A>
+__device__ __forceinline__ void norm_pitched(const Entry& e, uint64_t e0, uint64_t e1, A& acc) {
+    const T* p = static_cast<const T*>(e.in);
+    const uint64_t row = e0 / e.cols;
+    const uint32_t col = (uint32_t)(e0 - row * e.cols), count = (uint32_t)(e1 - e0);
+    p += row * e.in_pitch;
+    for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
+        const uint32_t at = col + i, r = at / e.cols;
+        acc.one(to_float(p[(uint64_t)r * e.in_pitch + (at - r * e.cols)]));
+    }
+}
+
+template <class T, class A>
+__device__ __forceinline__ void norm_part(const Entry& e, uint64_t e0, uint64_t e1, A& acc) {
+    if (e.cols) norm_pitched<T>(e, e0, e1, acc);
+    else norm_dense(static_cast<const T*>(e.in) + e0, e1 - e0, acc);
+}
+
+template <int NORM, int CAP>
+__global__ void __launch_bounds__(kThreads)
+qrc_k_list_norm(const __grid_constant__ Table<CAP> t, double* partials) {
+    wait_for_previous();
+    let_next_start();
+    Acc<NORM> acc;
+    for_share(t, blockIdx.x, gridDim.x, [&](const Entry& e, uint64_t e0, uint64_t e1) {
+        switch ((e.n_kind >> kKindShift) & 15) {
+            case QRC_F32: norm_part<float>(e, e0, e1, acc); break;
+            case QRC_BF16: norm_part<__nv_bfloat16>(e, e0, e1, acc); break;
+            default: norm_part<__half>(e, e0, e1, acc); break;
+        }
+    });
+    const double v = block_combine<NORM>(acc.value());
+    if (threadIdx.x == 0) partials[t.first_partial + blockIdx.x] = v;
+}
+
+// The norm from the partials: every block that calls it gets the same bits.
+template <int NORM> __device__ __forceinline__ double total_norm(const double* partials, uint32_t count) {
+    double v = 0.0;
+    for (uint32_t i = threadIdx.x; i < count; i += kThreads) v = combine<NORM>(v, partials[i]);
+    v = block_combine<NORM>(v);
+    return NORM == QRC_NORM_2 ? sqrt(v) : v;
+}
+
+template <int NORM>
+__global__ void __launch_bounds__(kThreads)
+qrc_k_list_finish(double* work, uint32_t count, float* norm) {
+    wait_for_previous();
+    let_next_start();
+    const double v = total_norm<NORM>(work + 1, count);
+    if (threadIdx.x == 0) {
+        work[0] = v;
+        if (norm) *norm = (float)v;
+    }
+}
+
+// -- clip ----------------------------------------------------------------------
+
+// NaN stays NaN, so a NaN norm shows in every output.
+__device__ __forceinline__ float clip_factor(double norm, double max_norm) {
+    if (isinf(max_norm)) return 1.0f;
+    const double k = max_norm / (norm + 1e-6);
+    return k >= 1.0 ? 1.0f : (float)k;
+}
+
+template <class TI, class TO>
+__device__ __forceinline__ void scale_vec(const uint4& v, void* out, float k) {
+    constexpr int VE = 16 / sizeof(TI), OB = VE * sizeof(TO);
+    float f[VE];
+    unpack<TI>(v, f);
+    __align__(16) TO r[VE];
+#pragma unroll
+    for (int i = 0; i < VE; i++) r[i] = from_float<TO>(f[i] * k);
+    if (OB == 8) *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(r);
+    else {
+#pragma unroll
+        for (int i = 0; i < OB / 16; i++) reinterpret_cast<uint4*>(out)[i] = reinterpret_cast<const uint4*>(r)[i];
+    }
+}
+
+template <class TI, class TO>
+__device__ __forceinline__ void scale_dense(const TI* p, TO* q, uint64_t n, float k) {
+    constexpr int VE = 16 / sizeof(TI), OB = VE * (int)sizeof(TO), OA = OB < 16 ? OB : 16, U = 4;
+    const uint64_t lead = ((16 - ((uintptr_t)p & 15)) & 15) / sizeof(TI);
+    const uint32_t head = (uint32_t)min(n, lead);
+    // Vectors need both sides aligned after the same number of elements;
+    // otherwise every element goes by itself.
+    if (((uintptr_t)(q + head) & (OA - 1)) != 0) {
+        for (uint64_t i = threadIdx.x; i < n; i += kThreads) q[i] = from_float<TO>(to_float(p[i]) * k);
+        return;
+    }
+    if (threadIdx.x < head) q[threadIdx.x] = from_float<TO>(to_float(p[threadIdx.x]) * k);
+    p += head;
+    q += head;
+    n -= head;
+    const uint4* v = reinterpret_cast<const uint4*>(p);
+    const uint32_t nv = (uint32_t)(n / VE);
+    uint32_t i = threadIdx.x;
+    for (; i + (U - 1) * kThreads < nv; i += U * kThreads) {
+        uint4 r[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) r[u] = v[i + u * kThreads];
+#pragma unroll
+        for (int u = 0; u < U; u++) scale_vec<TI, TO>(r[u], q + (uint64_t)(i + u * kThreads) * VE, k);
+    }
+    for (; i < nv; i += kThreads) scale_vec<TI, TO>(v[i], q + (uint64_t)i * VE, k);
+    const uint64_t done = (uint64_t)nv * VE;
+    if (threadIdx.x < (uint32_t)(n - done)) q[done + threadIdx.x] = from_float<TO>(to_float(p[done + threadIdx.x]) * k);
+}
+
+template <class TI, class TO>
+__device__ __forceinline__ void scale_part(const Entry& e, uint64_t e0, uint64_t e1, float k) {
+    const TI* p = static_cast<const TI*>(e.in);
+    TO* q = static_cast<TO*>(e.out);
+    if (!e.cols) return scale_dense(p + e0, q + e0, e1 - e0, k);
+    const uint64_t row = e0 / e.cols;
+    const uint32_t col = (uint32_t)(e0 - row * e.cols), count = (uint32_t)(e1 - e0);
+    p += row * e.in_pitch;
+    q += row * e.out_pitch;
+    for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
+        const uint32_t at = col + i, r = at / e.cols, c = at - r * e.cols;
+        q[(uint64_t)r * e.out_pitch + c] = from_float<TO>(to_float(p[(uint64_t)r * e.in_pitch + c]) * k);
+    }
+}
+
+template <class TI>
+__device__ __forceinline__ void scale_from(const Entry& e, uint64_t e0, uint64_t e1, float k) {
+    switch (e.n_kind >> (kKindShift + 4)) {
+        case QRC_F32: scale_part<TI, float>(e, e0, e1, k); break;
+        case QRC_BF16: scale_part<TI, __nv_bfloat16>(e, e0, e1, k); break;
+        default: scale_part<TI, __half>(e, e0, e1, k); break;
+    }
+}
+
+// `given` (a float norm in device memory) or work[0] decides the factor.  The
+// blocks walk the list from its end, which the norm pass read last.
+template <int CAP>
+__global__ void __launch_bounds__(kThreads)
+qrc_k_list_scale(const __grid_constant__ Table<CAP> t, const double* work, const float* given, double max_norm) {
+    wait_for_previous();
+    let_next_start();
+    const float k = clip_factor(given ? (double)*given : work[0], max_norm);
+    for_share(t, gridDim.x - 1 - blockIdx.x, gridDim.x, [&](const Entry& e, uint64_t e0, uint64_t e1) {
+        const int from = (int)(e.n_kind >> kKindShift) & 15, to = (int)(e.n_kind >> (kKindShift + 4));
+        if (k == 1.0f && e.in == e.out && from == to) return;       // x * 1 is what is there already
+        switch (from) {
+            case QRC_F32: scale_from<float>(e, e0, e1, k); break;
+            case QRC_BF16: scale_from<__nv_bfloat16>(e, e0, e1, k); break;
+            default: scale_from<__half>(e, e0, e1, k); break;
+        }
+    });
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+
+struct Launch {
+    std::vector<Entry> entries;
+    uint32_t chunks = 0, grid = 0, first_partial = 0;
+};
+
+inline uint64_t elem_bytes(int type) { return type == QRC_F32 ? 4 : 2; }
+
+// Memory that a tensor's input or output covers, from its first to its last byte.
+struct Extent {
+    uint64_t lo, hi;
+    uint64_t run, pitch;                      // bytes of a row and between rows' starts (pitch 0: dense)
+    uint32_t index;
+    bool out;
+};
+
+// True when the two share no byte for certain.
+bool disjoint(const Extent& a, const Extent& b) {
+    if (a.hi <= b.lo || b.hi <= a.lo) return true;
+    if (!a.pitch || a.pitch != b.pitch) return false;
+    // Rows at the same distance: apart when their columns are.
+    const uint64_t d = a.lo <= b.lo ? (b.lo - a.lo) % a.pitch : (a.pitch - (a.lo - b.lo) % a.pitch) % a.pitch;
+    return d >= a.run && d + b.run <= a.pitch;
+}
+
+bool same_place(const qrc_tensor& t) {
+    return t.d_in == t.d_out && t.in_type == t.out_type && (t.rows <= 1 || t.in_pitch == t.out_pitch);
+}
+
+// Whether every output element can be written without changing another
+// output or an input that some block has still to read.
+bool can_write(const std::vector<qrc_tensor>& ts) {
+    std::vector<Extent> all;
+    all.reserve(2 * ts.size());
+    for (uint32_t i = 0; i < ts.size(); i++) {
+        const qrc_tensor& t = ts[i];
+        if (!t.d_out) return false;
+        if (t.rows > 1 && t.out_pitch < t.cols) return false;         // rows written over each other
+        const uint64_t ib = elem_bytes(t.in_type), ob = elem_bytes(t.out_type);
+        const uint64_t in = (uintptr_t)t.d_in, out = (uintptr_t)t.d_out;
+        all.push_back({out, out + ((t.rows - 1) * t.out_pitch + t.cols) * ob, t.cols * ob,
+                       t.rows > 1 ? t.out_pitch * ob : 0, i, true});
+        if (!same_place(t))
+            all.push_back({in, in + ((t.rows - 1) * t.in_pitch + t.cols) * ib, t.cols * ib,
+                           t.rows > 1 ? t.in_pitch * ib : 0, i, false});
+    }
+    std::sort(all.begin(), all.end(), [](const Extent& a, const Extent& b) { return a.lo < b.lo; });
+    std::vector<Extent> open;
+    uint64_t compared = 0;
+    for (const Extent& e : all) {
+        open.erase(std::remove_if(open.begin(), open.end(), [&](const Extent& o) { return o.hi <= e.lo; }), open.end());
+        compared += open.size();
+        if (compared > (1ull << 26)) return false;                    // too entangled to prove
+        for (const Extent& o : open)
+            if ((o.out || e.out) && !disjoint(o, e)) return false;
+        open.push_back(e);
+    }
+    return true;
+}
+
+}  // namespace
+
+struct qrc_list {
+    int device = 0;
+    bool writable = false;
+    uint32_t partials = 0, chunk_log2 = kMaxChunkLog2;
+    std::vector<Launch> launches;
+};
+
+namespace {
+
+// Fills the plan; the tensors' arguments have been checked.
+void plan(qrc_list& l, const std::vector<qrc_tensor>& ts, int sms) {
+    uint64_t total = 0;
+    for (const qrc_tensor& t : ts) total += t.rows * t.cols * elem_bytes(t.in_type);
+    // Chunks of 32 KiB, smaller ones where they would leave SMs without work.
+    while (l.chunk_log2 > kMinChunkLog2 && (total >> l.chunk_log2) < 2u * sms) l.chunk_log2--;
+    for (const qrc_tensor& t : ts) {
+        const uint64_t n = t.rows * t.cols;
+        const uint64_t per = (1ull << l.chunk_log2) / elem_bytes(t.in_type), chunks = (n + per - 1) / per;
+        if (l.launches.empty() || l.launches.back().entries.size() == kLargeTable) l.launches.emplace_back();
+        Launch& a = l.launches.back();
+        const bool in_dense = t.rows <= 1 || t.in_pitch == t.cols;
+        const bool dense = in_dense && (!t.d_out || t.rows <= 1 || t.out_pitch == t.cols);
+        Entry e = {};
+        e.in = t.d_in;
+        e.out = t.d_out;
+        e.n_kind = n | (uint64_t)t.in_type << kKindShift | (uint64_t)t.out_type << (kKindShift + 4);
+        e.cols = dense ? 0 : (uint32_t)t.cols;
+        e.in_pitch = (uint32_t)t.in_pitch;
+        e.out_pitch = (uint32_t)t.out_pitch;
+        e.first = a.chunks;
+        a.entries.push_back(e);
+        a.chunks += (uint32_t)chunks;
+    }
+    for (Launch& a : l.launches) {
+        a.grid = std::min<uint32_t>(a.chunks, kMaxBlocks);
+        a.first_partial = l.partials;
+        l.partials += a.grid;
+    }
+}
+
+template <int CAP>
+void fill_table(Table<CAP>& t, const qrc_list& l, const Launch& a) {
+    std::memcpy(t.e, a.entries.data(), a.entries.size() * sizeof(Entry));
+    t.count = (uint32_t)a.entries.size();
+    t.chunks = a.chunks;
+    t.chunk_log2 = l.chunk_log2;
+    t.first_partial = a.first_partial;
+}
+
+template <int NORM, int CAP>
+cudaError_t launch_norm(const qrc_list& l, const Launch& a, double* work, cudaStream_t s) {
+    Table<CAP> t;
+    fill_table(t, l, a);
+    return launch_overlapped(qrc_k_list_norm<NORM, CAP>, dim3(a.grid), kThreads, 0, s, 1, t, work + 1);
+}
+
+template <int CAP>
+cudaError_t launch_scale(const qrc_list& l, const Launch& a, const double* work, const float* given, double max_norm,
+                         cudaStream_t s) {
+    Table<CAP> t;
+    fill_table(t, l, a);
+    return launch_overlapped(qrc_k_list_scale<CAP>, dim3(a.grid), kThreads, 0, s, 1, t, work, given, max_norm);
+}
+
+template <int NORM>
+cudaError_t run_norm(const qrc_list& l, double* work, float* norm, cudaStream_t s) {
+    for (const Launch& a : l.launches) {
+        const cudaError_t e = a.entries.size() <= kSmallTable ? launch_norm<NORM, kSmallTable>(l, a, work, s)
+                                                              : launch_norm<NORM, kLargeTable>(l, a, work, s);
+        if (e != cudaSuccess) return e;
+    }
+    return launch_overlapped(qrc_k_list_finish<NORM>, dim3(1), kThreads, 0, s, 1, work, l.partials, norm);
+}
+
+cudaError_t norm_by_order(const qrc_list& l, int norm, double* work, float* d_norm, cudaStream_t s) {
+    switch (norm) {
+        case QRC_NORM_1: return run_norm<QRC_NORM_1>(l, work, d_norm, s);
+        case QRC_NORM_2: return run_norm<QRC_NORM_2>(l, work, d_norm, s);
+        default: return run_norm<QRC_NORM_INF>(l, work, d_norm, s);
+    }
+}
+
+bool known_type(int t) { return t == QRC_F32 || t == QRC_BF16 || t == QRC_F16; }
+bool known_norm(int n) { return n == QRC_NORM_1 || n == QRC_NORM_2 || n == QRC_NORM_INF; }
+
+// Checks a caller's tensors and keeps those with elements.
+int checked(const qrc_tensor* tensors, size_t count, std::vector<qrc_tensor>& used) {
+    if (count && !tensors) return QRC_ERR_INVALID;
+    const uint64_t limit = 1ull << 40;
+    uint64_t total = 0;
+    for (size_t i = 0; i < count; i++) {
+        qrc_tensor t = tensors[i];
+        if (!known_type(t.in_type) || (t.d_out && !known_type(t.out_type))) return QRC_ERR_INVALID;
+        if (!t.d_out) t.out_type = t.in_type;
+        if (!t.rows || !t.cols) continue;
+        if (!t.d_in || ((uintptr_t)t.d_in & (elem_bytes(t.in_type) - 1)) ||
+            ((uintptr_t)t.d_out & (elem_bytes(t.out_type) - 1))) return QRC_ERR_INVALID;
+        if (t.rows > limit || t.cols > limit || t.rows > limit / t.cols) return QRC_ERR_RANGE;
+        const bool pitched = t.rows > 1 && (t.in_pitch != t.cols || (t.d_out && t.out_pitch != t.cols));
+        if (pitched && (t.cols >> 31 || t.in_pitch >> 32 || (t.d_out && t.out_pitch >> 32))) return QRC_ERR_RANGE;
+        total += t.rows * t.cols;
+        if (total > limit) return QRC_ERR_RANGE;
+        used.push_back(t);
+    }
+    return QRC_OK;
+}
+
+}  // namespace
+
+QRC_API int qrc_list_writable(const qrc_tensor* tensors, size_t count) {
+    std::vector<qrc_tensor> used;
+    int rc = QRC_OK;
+    try {
+        rc = checked(tensors, count, used);
+        return rc == QRC_OK ? (int)can_write(used) : rc;
+    } catch (const std::bad_alloc&) {
+        return QRC_ERR_RANGE;
+    }
+}
+
+QRC_API int qrc_list_create(qrc_list** out, int device, const qrc_tensor* tensors, size_t count) {
+    if (!out) return QRC_ERR_INVALID;
+    *out = nullptr;
+    try {
+        std::vector<qrc_tensor> used;
+        const int rc = checked(tensors, count, used);
+        if (rc != QRC_OK) return rc;
+        const int sms = sm100_sms(device);
+        if (!sms) return QRC_ERR_DEVICE;
+        qrc_list* l = new qrc_list();
+        try {
+            l->device = device;
+            plan(*l, used, sms);
+            l->writable = can_write(used);
+        } catch (...) {
+            delete l;
+            throw;
+        }
+        *out = l;
+    } catch (const std::bad_alloc&) {
+        return QRC_ERR_RANGE;
+    }
+    return QRC_OK;
+}
+
+QRC_API int qrc_list_destroy(qrc_list* l) {
+    delete l;
+    return QRC_OK;
+}
+
+QRC_API size_t qrc_list_workspace(const qrc_list* l) { return l ? (l->partials + 1) * sizeof(double) : 0; }
+
+QRC_API int qrc_list_norm(const qrc_list* l, int norm, float* d_norm, void* d_work, void* stream) {
+    if (!l || !d_norm || !d_work || !known_norm(norm)) return QRC_ERR_INVALID;
+    if (((uintptr_t)d_work & 7) || ((uintptr_t)d_norm & 3)) return QRC_ERR_INVALID;
+    DeviceScope scope(l->device);
+    if (!scope.ok) return QRC_ERR_STATE;
+    QRC_CK(norm_by_order(*l, norm, static_cast<double*>(d_work), d_norm, as_stream(stream)));
+    return QRC_OK;
+}
+
+QRC_API int qrc_list_clip(const qrc_list* l, int norm, double max_norm, const float* d_given, float* d_norm,
+                          void* d_work, void* stream) {
+    if (!l || !known_norm(norm) || !(max_norm >= 0.0) || !l->writable) return QRC_ERR_INVALID;
+    if (!d_given && (!d_work || ((uintptr_t)d_work & 7))) return QRC_ERR_INVALID;
+    if (((uintptr_t)d_given & 3) || ((uintptr_t)d_norm & 3)) return QRC_ERR_INVALID;
+    DeviceScope scope(l->device);
+    if (!scope.ok) return QRC_ERR_STATE;
+    cudaStream_t s = as_stream(stream);
+    double* work = static_cast<double*>(d_work);
+    if (!d_given) QRC_CK(norm_by_order(*l, norm, work, d_norm, s));
+    for (const Launch& a : l->launches)
+        QRC_CK(a.entries.size() <= kSmallTable ? launch_scale<kSmallTable>(*l, a, work, d_given, max_norm, s)
+                                               : launch_scale<kLargeTable>(*l, a, work, d_given, max_norm, s));
+    return QRC_OK;
+}

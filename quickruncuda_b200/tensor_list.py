@@ -1,0 +1,188 @@
+"""One norm over many tensors, and scaling them by it: the gradient norm and
+gradient clipping of a training step (qrc_list_* of include/qrc_b200.h).
+
+    grads = q.TensorList([p.grad for p in params])
+    norm = grads.clip_norm(1.0)          # scales in place, returns the norm before
+
+A `TensorList` is a plan: it is made once, keeps the tensors alive and can be
+used from any stream, thread or captured graph.  It holds the tensors it was
+given: gradients that a later step allocates anew need a new list (with
+`zero_grad(set_to_none=False)` they stay where they are).
+"""
+from __future__ import annotations
+
+import ctypes
+import itertools
+import math
+from typing import Optional, Sequence
+
+import torch
+
+from . import _native as nat
+from .api import _empty, _stream_handle
+
+_TYPES = {torch.float32: nat.TYPE_F32, torch.bfloat16: nat.TYPE_BF16, torch.float16: nat.TYPE_F16}
+_NORMS = {1.0: nat.NORM_1, 2.0: nat.NORM_2, math.inf: nat.NORM_INF}
+
+# A tensor that is neither dense nor rows at one distance is taken apart into
+# pieces that are; with more of them than this it is refused.
+MAX_PIECES = 4096
+
+
+def _pieces(shape, strides, out_strides):
+    """Splits a strided tensor (and an output of the same shape) into runs of
+    rows: yields (offset, out offset, rows, cols, pitch, out pitch), in
+    elements.  The elements of one piece are neighbours in both."""
+    dims = [(n, s, o) for n, s, o in zip(shape, strides, out_strides) if n != 1]
+    if any(n == 0 for n, _, _ in dims):
+        return []
+    dims.sort(key=lambda d: (d[1], d[2]), reverse=True)
+    joined = []
+    for n, s, o in dims:
+        if joined and joined[-1][1] == s * n and joined[-1][2] == o * n:
+            n, _, _ = (joined.pop()[0] * n, s, o)
+        joined.append((n, s, o))
+    if not joined or joined[-1][1] != 1 or joined[-1][2] != 1:
+        joined.append((1, 1, 1))                    # no run of neighbours: columns of one
+    cols = joined.pop()[0]
+    rows, pitch, out_pitch = joined.pop() if joined else (1, cols, cols)
+    if math.prod(n for n, _, _ in joined) > MAX_PIECES:
+        raise RuntimeError(f"TensorList: a tensor of shape {tuple(shape)} and strides {tuple(strides)} falls into "
+                           f"more than {MAX_PIECES} pieces; make it contiguous")
+    return [(sum(i * s for i, (_, s, _) in zip(at, joined)), sum(i * o for i, (_, _, o) in zip(at, joined)),
+             rows, cols, pitch, out_pitch)
+            for at in itertools.product(*(range(n) for n, _, _ in joined))]
+
+
+def _describe(tensors: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]]):
+    """The qrc_tensor array of a list and its device index (None when empty)."""
+    if out is not None and len(out) != len(tensors):
+        raise RuntimeError(f"TensorList: {len(tensors)} tensors but {len(out)} outputs")
+    device, rows = None, []
+    for i, x in enumerate(tensors):
+        y = x if out is None else out[i]
+        for t in (x,) if y is x else (x, y):
+            if t.device.type != "cuda":
+                raise RuntimeError(f"TensorList needs CUDA tensors, got one on {t.device}")
+            if t.dtype not in _TYPES:
+                raise RuntimeError(f"TensorList needs dtypes in {tuple(_TYPES)}, got {t.dtype}")
+            if t.layout != torch.strided:
+                raise RuntimeError(f"TensorList needs strided tensors, got {t.layout}")
+            if device is None:
+                device = t.device
+            elif t.device != device:
+                raise RuntimeError(f"TensorList needs tensors of one device, got {device} and {t.device}")
+        if x.shape != y.shape:
+            raise RuntimeError(f"TensorList: an output of shape {tuple(y.shape)} for a tensor of shape {tuple(x.shape)}")
+        xt, yt, xp, yp = _TYPES[x.dtype], _TYPES[y.dtype], x.data_ptr(), y.data_ptr()
+        n = x.numel()
+        if x.is_contiguous() and (y is x or y.is_contiguous()):
+            rows.append((xp, yp, 1, n, n, n, xt, yt))
+            continue
+        xs, ys = x.element_size(), y.element_size()
+        rows += [(xp + a * xs, yp + b * ys, r, c, p, q, xt, yt)
+                 for a, b, r, c, p, q in _pieces(x.shape, x.stride(), y.stride())]
+    return (nat.Tensor * len(rows))(*rows), None if device is None else device.index
+
+
+class TensorList:
+    """A plan over CUDA tensors of float32, bfloat16 and float16, in any mix,
+    of any strides, all on one device.  `out` (tensors of the same shapes, any
+    of the three types) receives what `clip_norm` scales; without it the
+    tensors are scaled in place."""
+
+    def __init__(self, tensors: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]] = None,
+                 device: Optional[int] = None):
+        self.lib = nat.load()
+        self.tensors = list(tensors)
+        self.out = self.tensors if out is None else list(out)
+        table, index = _describe(self.tensors, None if out is None else self.out)
+        if index is None:
+            index = torch.cuda.current_device() if device is None else int(device)
+        elif device is not None and int(device) != index:
+            raise RuntimeError(f"TensorList for device {device} got tensors on cuda:{index}")
+        self.device = index
+        h = ctypes.c_void_p()
+        nat.check(self.lib, "qrc_list_create", self.lib.qrc_list_create(ctypes.byref(h), index, table, len(table)))
+        self._h = h
+        self._work_bytes = int(self.lib.qrc_list_workspace(h))
+        # 1 when the outputs can be written without one changing another
+        self._writable = self.lib.qrc_list_writable(table, len(table)) == 1
+        self._torch_device = torch.device("cuda", index)
+
+    def close(self) -> None:
+        if getattr(self, "_h", None) is not None:
+            self.lib.qrc_list_destroy(self._h)
+            self._h = None
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    @property
+    def handle(self) -> ctypes.c_void_p:
+        if self._h is None:
+            raise RuntimeError("list closed")
+        return self._h
+
+    def __len__(self) -> int:
+        return len(self.tensors)
+
+    def _scalar(self, t, name: str) -> torch.Tensor:
+        if t.device != self._torch_device or t.dtype != torch.float32 or t.numel() != 1:
+            raise RuntimeError(f"TensorList: {name} has to be one float32 on {self._torch_device}, "
+                               f"got {tuple(t.shape)} {t.dtype} on {t.device}")
+        return t
+
+    @staticmethod
+    def _order(ord) -> int:
+        code = _NORMS.get(float(ord))
+        if code is None:
+            raise RuntimeError(f"TensorList: the norm is of order 1, 2 or inf, got {ord!r}")
+        return code
+
+    def norm(self, ord: float = 2.0, out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+        """The norm over all elements of all tensors, a float32 tensor (0-dim,
+        or `out`).  ord 1: sum |x|, 2: sqrt(sum x^2), inf: max |x|, summed in
+        float64; a NaN element gives NaN.  The same bits on every call.
+        Asynchronous."""
+        code = self._order(ord)
+        out = _empty((), torch.float32, self._torch_device, stream) if out is None else self._scalar(out, "out")
+        work = _empty(self._work_bytes, torch.uint8, self._torch_device, stream)
+        nat.check(self.lib, "qrc_list_norm",
+                  self.lib.qrc_list_norm(self.handle, code, out.data_ptr(), work.data_ptr(),
+                                         _stream_handle(stream, self.device) or None))
+        return out
+
+    def clip_norm(self, max_norm: float, ord: float = 2.0, norm: Optional[torch.Tensor] = None,
+                  stream=None) -> torch.Tensor:
+        """Scales every tensor by min(1, max_norm / (norm + 1e-6)) into its
+        output and returns the norm from before.  `norm` (one float32 on the
+        device) stands in for the list's own, for instance a norm over the
+        shards of several GPUs.  Asynchronous, nothing is read back."""
+        code = self._order(ord)
+        max_norm = float(max_norm)
+        if not max_norm >= 0.0:
+            raise RuntimeError(f"TensorList: max_norm has to be 0 or more, got {max_norm}")
+        if not self._writable:
+            raise RuntimeError("TensorList: outputs share memory with one another or with other tensors; "
+                               "scaling them would change elements twice")
+        given = 0
+        if norm is not None:
+            given, result, work = self._scalar(norm, "norm").data_ptr(), norm, None
+        else:
+            result = _empty((), torch.float32, self._torch_device, stream)
+            work = _empty(self._work_bytes, torch.uint8, self._torch_device, stream)
+        nat.check(self.lib, "qrc_list_clip",
+                  self.lib.qrc_list_clip(self.handle, code, max_norm, given or None, result.data_ptr(),
+                                         work.data_ptr() if work is not None else None,
+                                         _stream_handle(stream, self.device) or None))
+        return result

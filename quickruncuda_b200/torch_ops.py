@@ -1,5 +1,7 @@
 """PyTorch custom operators over the C ABI: `torch.ops.qrc.absmax`,
-`torch.ops.qrc.reduce` and `torch.ops.qrc.amax_quant_e4m3`.
+`torch.ops.qrc.reduce` and `torch.ops.qrc.amax_quant_e4m3`; for gradients
+`torch.ops.qrc.grad_norm` and `torch.ops.qrc.clip_grad_norm_`; for 4-bit
+weights `torch.ops.qrc.quant_w4`, `dequant_w4` and `matvec_w4`.
 
 These are for callers that hold tensors rather than raw buffers, such as a
 quantized-inference stack computing per-tensor FP8 scales.  They are opaque
@@ -19,10 +21,13 @@ from __future__ import annotations
 
 import collections
 import threading
+from typing import List, Optional
 
 import torch
 
 from .api import SideAwareContext
+from .tensor_list import TensorList
+from .weight4 import Weight4, packed_shape, quant_w4 as _quant_w4
 
 _CACHE_PER_DEVICE = 16
 _cache: "collections.OrderedDict[tuple, SideAwareContext]" = collections.OrderedDict()
@@ -124,3 +129,80 @@ def amax_quant_e4m3(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor, torch.
 def _(x: torch.Tensor):
     return (x.new_empty(x.shape, dtype=torch.float8_e4m3fn), x.new_empty((), dtype=torch.float32),
             x.new_empty((), dtype=torch.float32))
+
+
+# -- gradients of a training step ------------------------------------------------
+
+@torch.library.custom_op("qrc::grad_norm", mutates_args=(), device_types="cuda")
+def grad_norm(grads: List[torch.Tensor], ord: float = 2.0) -> torch.Tensor:
+    """The norm (ord 1, 2 or inf) over all elements of all tensors, 0-dim
+    float32; see TensorList, which saves making the plan on every call."""
+    with TensorList(grads) as tensors:
+        return tensors.norm(ord)
+
+
+@grad_norm.register_fake
+def _(grads: List[torch.Tensor], ord: float = 2.0) -> torch.Tensor:
+    return grads[0].new_empty((), dtype=torch.float32)
+
+
+@torch.library.custom_op("qrc::clip_grad_norm_", mutates_args=("grads",), device_types="cuda")
+def clip_grad_norm_(grads: List[torch.Tensor], max_norm: float, ord: float = 2.0) -> torch.Tensor:
+    """Scales the tensors in place by min(1, max_norm / (norm + 1e-6)) and
+    returns the norm from before, 0-dim float32."""
+    with TensorList(grads) as tensors:
+        return tensors.clip_norm(max_norm, ord)
+
+
+@clip_grad_norm_.register_fake
+def _(grads: List[torch.Tensor], max_norm: float, ord: float = 2.0) -> torch.Tensor:
+    return grads[0].new_empty((), dtype=torch.float32)
+
+
+# -- 4-bit weights ----------------------------------------------------------------
+
+@torch.library.custom_op("qrc::quant_w4", mutates_args=(), device_types="cuda")
+def quant_w4(w: torch.Tensor, group: int = 128, symmetric: bool = True) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(packed, scales, zeros) of a bfloat16 or float16 matrix, as in Weight4;
+    zeros has no elements when symmetric."""
+    w4 = _quant_w4(w, group=group, symmetric=symmetric)
+    zeros = w4.zeros if w4.zeros is not None else torch.empty(0, dtype=torch.uint8, device=w.device)
+    return w4.packed, w4.scales, zeros
+
+
+@quant_w4.register_fake
+def _(w: torch.Tensor, group: int = 128, symmetric: bool = True):
+    n, k = w.shape
+    groups = (-(-k // group), n)
+    return (w.new_empty(packed_shape(n, k), dtype=torch.int32), w.new_empty(groups),
+            w.new_empty((0,) if symmetric else groups, dtype=torch.uint8))
+
+
+def _weight4(packed, scales, zeros, k: int, group: int) -> Weight4:
+    return Weight4(packed, scales, None if zeros is None or zeros.shape != scales.shape and zeros.numel() == 0 else zeros,
+                   k, group)
+
+
+@torch.library.custom_op("qrc::dequant_w4", mutates_args=(), device_types="cuda")
+def dequant_w4(packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], k: int, group: int,
+               dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """The values [n, k] of a 4-bit matrix (zeros None or empty: symmetric)."""
+    return _weight4(packed, scales, zeros, k, group).dequant(dtype=dtype)
+
+
+@dequant_w4.register_fake
+def _(packed, scales, zeros, k: int, group: int, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    return scales.new_empty((packed.shape[0], k), dtype=scales.dtype if dtype is None else dtype)
+
+
+@torch.library.custom_op("qrc::matvec_w4", mutates_args=(), device_types="cuda")
+def matvec_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], group: int,
+              bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """x [..., k] times a 4-bit matrix [n, k] (+ bias): [..., n], see
+    Weight4.matvec (zeros None or empty: symmetric)."""
+    return _weight4(packed, scales, zeros, x.shape[-1], group).matvec(x, bias=bias, out_dtype=out_dtype)
+
+
+@matvec_w4.register_fake
+def _(x, packed, scales, zeros, group: int, bias=None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    return x.new_empty(x.shape[:-1] + (packed.shape[0],), dtype=x.dtype if out_dtype is None else out_dtype)

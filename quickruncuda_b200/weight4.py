@@ -1,0 +1,180 @@
+"""Weight matrices in 4 bits with one scale per group of columns: quantize,
+dequantize and the product with a few rows of activations (qrc_w4_* of
+include/qrc_b200.h).
+
+    w4 = q.quant_w4(w, group=128)        # w bfloat16 or float16 [n, k]
+    y = w4.matvec(x)                     # x [..., k] -> y [..., n]
+
+    value[n][k] = (code[n][k] - zero[g][n]) * scale[g][n],  g = k // group
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional
+
+import torch
+
+from . import _native as nat
+from .api import _empty, _stream_handle
+
+_TYPES = {torch.bfloat16: nat.TYPE_BF16, torch.float16: nat.TYPE_F16}
+_OUT_TYPES = {torch.float32: nat.TYPE_F32, **_TYPES}
+GROUPS = (32, 64, 128, 256)
+
+
+def _check(t: torch.Tensor, name: str, dtypes, shape=None, device=None) -> None:
+    if t.device.type != "cuda":
+        raise RuntimeError(f"Weight4: {name} has to be a CUDA tensor, got {t.device}")
+    if device is not None and t.device != device:
+        raise RuntimeError(f"Weight4: {name} has to be on {device}, got {t.device}")
+    if t.dtype not in dtypes:
+        raise RuntimeError(f"Weight4: {name} needs dtype in {tuple(dtypes)}, got {t.dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise RuntimeError(f"Weight4: {name} has shape {tuple(t.shape)}, needs {tuple(shape)}")
+
+
+def _pitch(t: torch.Tensor, name: str) -> int:
+    """Elements between the rows of a 2-D tensor whose rows are runs of
+    neighbouring elements that do not overlap."""
+    rows, cols = t.shape
+    if cols > 1 and t.stride(1) != 1 or rows > 1 and t.stride(0) < cols:
+        raise RuntimeError(f"Weight4: {name} needs rows of neighbouring elements, got strides {t.stride()}")
+    return t.stride(0) if rows > 1 else cols
+
+
+def _check_group(group: int) -> int:
+    if group not in GROUPS:
+        raise RuntimeError(f"Weight4: group has to be one of {GROUPS}, got {group!r}")
+    return int(group)
+
+
+def packed_shape(n: int, k: int):
+    return (n, -(-k // 128) * 16)
+
+
+class Weight4:
+    """A 4-bit weight matrix of n rows (outputs) and k columns (inputs).
+
+    packed  int32 [n, ceil(k / 128) * 16], codes in the order of qrc_b200.h
+    scales  bfloat16 or float16 [ceil(k / group), n]
+    zeros   uint8 [ceil(k / group), n] of 0..15, or None: all 8
+
+    The constructor takes tensors that are laid out so already (a saved
+    matrix); `quant_w4` and `from_codes` make new ones."""
+
+    def __init__(self, packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor], k: int, group: int):
+        group, k = _check_group(group), int(k)
+        if k < 0:
+            raise RuntimeError(f"Weight4: k has to be 0 or more, got {k}")
+        n = int(packed.shape[0]) if packed.dim() else 0
+        _check(packed, "packed", (torch.int32,), packed_shape(n, k))
+        groups = (-(-k // group), n)
+        _check(scales, "scales", _TYPES, groups, packed.device)
+        if zeros is not None:
+            _check(zeros, "zeros", (torch.uint8,), groups, packed.device)
+        for name, t in (("packed", packed), ("scales", scales), ("zeros", zeros)):
+            if t is not None and not t.is_contiguous():
+                raise RuntimeError(f"Weight4: {name} has to be contiguous")
+        self.lib = nat.load()
+        self.packed, self.scales, self.zeros = packed, scales, zeros
+        self.shape, self.group, self.dtype, self.device = (n, k), group, scales.dtype, packed.device
+        self._w = nat.W4(packed.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(), n, k, group,
+                         _TYPES[scales.dtype])
+        self._ref = ctypes.byref(self._w)
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
+                   group: int = 128, stream=None) -> "Weight4":
+        """Packs codes held one per byte (uint8 [n, k], the low four bits
+        count).  `scales` and `zeros` as in the class, kept as they are."""
+        _check(codes, "codes", (torch.uint8,))
+        if codes.dim() != 2:
+            raise RuntimeError(f"Weight4: codes have to be 2-D, got {tuple(codes.shape)}")
+        n, k = codes.shape
+        ld = _pitch(codes, "codes")
+        w4 = cls(_empty(packed_shape(n, k), torch.int32, codes.device, stream), scales, zeros, k, group)
+        nat.check(w4.lib, "qrc_w4_pack",
+                  w4.lib.qrc_w4_pack(codes.device.index, codes.data_ptr(), ld, w4._ref,
+                                     _stream_handle(stream, codes.device.index) or None))
+        return w4
+
+    def dequant(self, out: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None,
+                stream=None) -> torch.Tensor:
+        """The values, [n, k] of `dtype` (the scales' type by default; float32
+        holds them exactly).  Asynchronous."""
+        if out is None:
+            dtype = self.dtype if dtype is None else dtype
+            if dtype not in _OUT_TYPES:
+                raise RuntimeError(f"Weight4: dequant needs dtype in {tuple(_OUT_TYPES)}, got {dtype}")
+            out = _empty(self.shape, dtype, self.device, stream)
+        else:
+            _check(out, "out", _OUT_TYPES if dtype is None else (dtype,), self.shape, self.device)
+        nat.check(self.lib, "qrc_w4_dequant",
+                  self.lib.qrc_w4_dequant(self.device.index, self._ref, out.data_ptr(), _pitch(out, "out"),
+                                          _OUT_TYPES[out.dtype], _stream_handle(stream, self.device.index) or None))
+        return out
+
+    def matvec(self, x: torch.Tensor, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+               out_dtype: Optional[torch.dtype] = None, stream=None) -> torch.Tensor:
+        """x @ values.T (+ bias) for x [..., k] of the scales' type: y [..., n]
+        of that type or, with out_dtype, of float32.  Made for a few rows (a
+        decode step).  Sums in float32.  Asynchronous."""
+        n, k = self.shape
+        _check(x, "x", (self.dtype,), device=self.device)
+        if x.dim() == 0 or x.shape[-1] != k:
+            raise RuntimeError(f"Weight4: x has shape {tuple(x.shape)}, needs [..., {k}]")
+        if bias is not None:
+            _check(bias, "bias", (self.dtype,), (n,), self.device)
+            if n > 1 and bias.stride(0) != 1:
+                raise RuntimeError("Weight4: bias has to be contiguous")
+        shape = x.shape[:-1] + (n,)
+        kind = out_dtype if out_dtype is not None else out.dtype if out is not None else self.dtype
+        if kind != torch.float32 and kind != self.dtype:
+            raise RuntimeError(f"Weight4: matvec gives {self.dtype} or float32, got {kind}")
+        if out is None:
+            out = _empty(shape, kind, self.device, stream)
+        else:
+            _check(out, "out", (kind,), shape, self.device)
+        m = x.numel() // k if k else shape[:-1].numel()
+        x2 = _as_rows(x, m, k, "x")
+        y2 = _as_rows(out, m, n, "out")
+        ldx, ldy = _pitch(x2, "x"), _pitch(y2, "out")
+        need = self.lib.qrc_w4_matvec_workspace(self._ref, x.data_ptr(), m, ldx)
+        work = _empty(need, torch.uint8, self.device, stream) if need else None
+        nat.check(self.lib, "qrc_w4_matvec",
+                  self.lib.qrc_w4_matvec(self.device.index, self._ref, x.data_ptr(), m, ldx,
+                                         None if bias is None else bias.data_ptr(), out.data_ptr(), ldy,
+                                         _OUT_TYPES[kind], None if work is None else work.data_ptr(),
+                                         _stream_handle(stream, self.device.index) or None))
+        return out
+
+
+def _as_rows(t: torch.Tensor, rows: int, cols: int, name: str) -> torch.Tensor:
+    """A 2-D view of t over its last dimension."""
+    if t.dim() == 2:
+        return t
+    try:
+        return t.view(rows, cols)
+    except RuntimeError:
+        raise RuntimeError(f"Weight4: {name} of shape {tuple(t.shape)} and strides {t.stride()} is not rows at one "
+                           "distance; make it contiguous") from None
+
+
+def quant_w4(w: torch.Tensor, group: int = 128, symmetric: bool = True, stream=None) -> Weight4:
+    """Quantizes a bfloat16 or float16 CUDA matrix [n, k] to 4 bits with one
+    scale per row and group of columns.  symmetric: scale = max |x| / 7, codes
+    around 8; otherwise scale = (max - min) / 15 over the group and 0, with a
+    zero point.  NaN gives 0, infinities the end of their group's range.
+    Asynchronous."""
+    _check(w, "w", _TYPES)
+    if w.dim() != 2:
+        raise RuntimeError(f"Weight4: w has to be 2-D, got {tuple(w.shape)}")
+    n, k = w.shape
+    ld = _pitch(w, "w")
+    groups = (-(-k // _check_group(group)), n)
+    w4 = Weight4(_empty(packed_shape(n, k), torch.int32, w.device, stream), _empty(groups, w.dtype, w.device, stream),
+                 None if symmetric else _empty(groups, torch.uint8, w.device, stream), k, group)
+    nat.check(w4.lib, "qrc_w4_quant",
+              w4.lib.qrc_w4_quant(w.device.index, w.data_ptr(), ld, int(bool(symmetric)), w4._ref,
+                                  _stream_handle(stream, w.device.index) or None))
+    return w4

@@ -1,0 +1,153 @@
+"""Lists of tensors (quickruncuda_b200/tensor_list.py, qrc_list_*) without a
+GPU: how strided tensors are taken apart, which outputs may be written, and
+what is refused before any GPU work."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+import quickruncuda_b200 as q
+import quickruncuda_b200.torch_ops  # noqa: F401  (registers torch.ops.qrc.*)
+from quickruncuda_b200 import _native as nat
+from quickruncuda_b200 import tensor_list
+from quickruncuda_b200.tensor_list import _pieces
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+
+def _views():
+    base = torch.arange(2 * 6 * 10 * 4)
+    b4 = base.view(2, 6, 10, 4)
+    return [base, b4, b4[:, :, 2:9], b4[..., 1:3], b4[..., ::2], b4.permute(3, 1, 0, 2), b4[:, 3], b4[1, :, :, 2],
+            b4[:, :, :, :1], b4.transpose(1, 2)[..., 3:], base[7:8], base[5:5], b4[:, :0], base[3].view(()),
+            b4[:, ::2, ::3], b4.to(memory_format=torch.channels_last)]
+
+
+@pytest.mark.parametrize("i", range(16))
+def test_pieces_visit_every_element_once_and_in_step(i):
+    x = _views()[i]
+    flat = torch.as_strided(x, (x.untyped_storage().nbytes() // x.element_size(),), (1,), 0)
+    for y in (x, torch.empty(x.shape)):
+        seen = []
+        for a, b, rows, cols, pitch, out_pitch in _pieces(x.shape, x.stride(), y.stride()):
+            for r in range(rows):
+                for c in range(cols):
+                    at = a + r * pitch + c
+                    seen.append((int(flat[x.storage_offset() + at]), b + r * out_pitch + c))
+        # the same walk through indices: value at every output offset
+        want = []
+        index = torch.cartesian_prod(*[torch.arange(n) for n in x.shape]).view(-1, x.dim()) if x.dim() else torch.zeros(1, 0)
+        for at in index.tolist() if x.numel() else []:
+            want.append((int(x[tuple(int(v) for v in at)]), sum(int(v) * s for v, s in zip(at, y.stride()))))
+        assert sorted(seen) == sorted(want)
+
+
+def test_dense_tensors_are_one_piece():
+    for x in (torch.empty(5, 7), torch.empty(7, 5).t(), torch.empty(2, 3, 4, 5).permute(2, 0, 3, 1), torch.empty(())):
+        assert len(_pieces(x.shape, x.stride(), x.stride())) == 1
+    assert len(_pieces((4, 6), (9, 1), (9, 1))) == 1            # rows at one distance
+    assert _pieces((4, 0), (9, 1), (9, 1)) == []
+
+
+def test_too_many_pieces_are_refused():
+    # three dimensions of which none joins another, nor has neighbours: 50 * 50
+    # pieces of 50 rows of one element
+    x = torch.empty(99, 99, 99)[::2, ::2, ::2]
+    assert len(_pieces(x.shape, x.stride(), x.stride())) == 2500
+    y = torch.empty(199, 99, 99)[::2, ::2, ::2]         # 100 * 50
+    with pytest.raises(RuntimeError, match="make it contiguous"):
+        _pieces(y.shape, y.stride(), y.stride())
+
+
+def _writable(*tensors):
+    table = (nat.Tensor * len(tensors))(*tensors)
+    return nat.load().qrc_list_writable(table, len(tensors))
+
+
+def _t(at, to, n=None, rows=1, cols=None, pitch=0, out_pitch=None, kind=0, out_kind=None):
+    return (at, to, rows, cols if cols is not None else n, pitch, pitch if out_pitch is None else out_pitch, kind,
+            kind if out_kind is None else out_kind)
+
+
+def test_writable():
+    A, B = 1 << 20, 1 << 21
+    assert _writable() == 1
+    assert _writable(_t(A, A, 100)) == 1                                    # in place
+    assert _writable(_t(A, B, 100)) == 1                                    # into another
+    assert _writable(_t(A, None, 100)) == 0                                 # no output
+    assert _writable(_t(A, A, 100), _t(A, A, 100)) == 0                     # the same tensor twice
+    assert _writable(_t(A, A, 100), _t(A + 400, A + 400, 100)) == 1         # neighbours
+    assert _writable(_t(A, A, 100), _t(A + 396, A + 396, 100)) == 0         # one element shared
+    assert _writable(_t(A, A + 4, 100)) == 0                                # shifted onto itself
+    assert _writable(_t(A, B, 100), _t(A, B + 400, 100)) == 1               # one input, two outputs
+    assert _writable(_t(A, B, 100), _t(B, A + 4096, 100)) == 0              # writes what another reads
+    assert _writable(_t(A, A, 100, kind=1, out_kind=2)) == 0                # in place, other type
+    assert _writable(_t(A, A, 100, kind=1, out_kind=0)) == 0
+    # column slices of one buffer, 40 columns: apart, then one column shared
+    left = _t(A, A, rows=50, cols=16, pitch=40)
+    assert _writable(left, _t(A + 64, A + 64, rows=50, cols=24, pitch=40)) == 1
+    assert _writable(left, _t(A + 60, A + 60, rows=50, cols=24, pitch=40)) == 0
+    assert _writable(_t(A + 64, A + 64, rows=50, cols=24, pitch=40), left) == 1
+    assert _writable(left, _t(A + 64, A + 64, rows=50, cols=25, pitch=40)) == 0   # runs into the next row
+    assert _writable(left, _t(A + 64, A + 64, rows=2, cols=4, pitch=44)) == 0     # other distance: not shown
+    assert _writable(_t(A, A, rows=50, cols=16, pitch=15)) == 0             # rows on top of each other
+    assert _writable(_t(A, A, rows=50, cols=16, pitch=0)) == 0              # one row, repeated
+    assert _writable(_t(A, B, rows=50, cols=16, pitch=0, out_pitch=16)) == 1
+    assert _writable(_t(A, A, 0), _t(A, A, 0)) == 1                         # nothing to write
+
+
+def test_c_refusals(lib):
+    A = 1 << 20
+    h = ctypes.c_void_p()
+
+    def create(*tensors):
+        return lib.qrc_list_create(ctypes.byref(h), 0, (nat.Tensor * len(tensors))(*tensors), len(tensors))
+
+    assert lib.qrc_list_create(None, 0, None, 0) == nat.QRC_ERR_INVALID
+    assert lib.qrc_list_create(ctypes.byref(h), 0, None, 1) == nat.QRC_ERR_INVALID
+    assert create(_t(A, A, 4, kind=3)) == nat.QRC_ERR_INVALID
+    assert create(_t(A, A, 4, kind=0, out_kind=-1)) == nat.QRC_ERR_INVALID
+    assert create(_t(None, A, 4)) == nat.QRC_ERR_INVALID
+    assert create(_t(A + 2, A, 4)) == nat.QRC_ERR_INVALID
+    assert create(_t(A, A + 1, 4, kind=1)) == nat.QRC_ERR_INVALID
+    assert create(_t(A, A, (1 << 40) + 1)) == nat.QRC_ERR_RANGE
+    assert create(_t(A, A, 1 << 40), _t(A, A, 1)) == nat.QRC_ERR_RANGE
+    assert create(_t(A, A, rows=1 << 21, cols=1 << 21, pitch=1 << 21)) == nat.QRC_ERR_RANGE
+    assert create(_t(A, A, rows=2, cols=4, pitch=1 << 32)) == nat.QRC_ERR_RANGE
+    assert h.value is None
+    assert lib.qrc_list_destroy(None) == 0
+    assert lib.qrc_list_workspace(None) == 0
+    assert lib.qrc_list_norm(None, 2, A, A, None) == nat.QRC_ERR_INVALID
+    assert lib.qrc_list_clip(None, 2, 1.0, None, A, A, None) == nat.QRC_ERR_INVALID
+
+
+def test_python_refusals():
+    with pytest.raises(RuntimeError, match="CUDA tensors"):
+        q.TensorList([torch.ones(3)])
+    with pytest.raises(RuntimeError, match="2 tensors but 1 outputs"):
+        q.TensorList([torch.ones(3)] * 2, out=[torch.ones(3)])
+    for bad in (3.0, 0.0, -1.0, math.nan):
+        with pytest.raises(RuntimeError, match="order 1, 2 or inf"):
+            q.TensorList._order(bad)
+    assert q.TensorList._order(2) == nat.NORM_2 and q.TensorList._order(math.inf) == nat.NORM_INF
+    with FakeTensorMode():
+        x = torch.empty(3, device="cuda")
+        with pytest.raises(RuntimeError, match="dtypes"):
+            tensor_list._describe([x.double()], None)
+        with pytest.raises(RuntimeError, match="shape"):
+            tensor_list._describe([x], [torch.empty(4, device="cuda")])
+        with pytest.raises(RuntimeError, match="one device"):
+            tensor_list._describe([x, torch.empty(3, device="cuda:1")], None)
+        with pytest.raises(RuntimeError, match="CUDA tensors"):
+            tensor_list._describe([x], [torch.empty(3)])
+
+
+def test_operators_registered():
+    with FakeTensorMode():
+        x = [torch.empty(3, 5, device="cuda"), torch.empty(7, device="cuda", dtype=torch.bfloat16)]
+        for y in (torch.ops.qrc.grad_norm(x), torch.ops.qrc.grad_norm(x, math.inf), torch.ops.qrc.clip_grad_norm_(x, 1.0)):
+            assert y.shape == () and y.dtype == torch.float32 and y.device.type == "cuda"
+    with pytest.raises(NotImplementedError):
+        torch.ops.qrc.grad_norm([torch.ones(3)])
+    with pytest.raises(NotImplementedError):
+        torch.ops.qrc.clip_grad_norm_([torch.ones(3)], 1.0)

@@ -1,0 +1,329 @@
+"""The norm over a list of tensors and scaling by it, against the formulas in
+64 bits.
+
+Tolerances, relative, u = 2^-24 (half a step of float32):
+  L2    1.5 u: the result's rounding, and sums in double (n * 2^-53 < u / 4 for
+        n < 2^27).  16-bit inputs add up eight terms in float first, 7 u of a
+        sum of non-negative terms at most, half of it after the root: 5 u.
+  L1    1.5 u; 16-bit inputs 8.5 u.
+  Linf  exact.
+  clip  the factor's rounding u and the product's u, plus what the norm may be
+        off (5 u or 8.5 u at most: 11 u together), then half a step of the
+        output's type: eps / 2 of the value, or half of its smallest number.
+"""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+ORDS = [1.0, 2.0, math.inf]
+
+
+def _types():
+    import torch
+    return {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def _make(sizes, kinds, seed=0, scale=1.0):
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return [torch.randn(s, generator=gen, device="cuda").mul_(scale * 2.0 ** -(i % 5)).to(_types()[k])
+            for i, (s, k) in enumerate(zip(sizes, kinds))]
+
+
+def _exact(tensors, ord):
+    import torch
+    total = torch.zeros((), dtype=torch.float64, device="cuda")
+    for t in tensors:
+        d = t.double().abs().flatten()
+        if not d.numel():
+            continue
+        if ord == math.inf:
+            total = torch.maximum(total, d.max())
+        else:
+            total = total + (d if ord == 1.0 else d * d).sum()
+    return float(total.sqrt() if ord == 2.0 else total)
+
+
+def _tolerance(tensors, ord):
+    if ord == math.inf:
+        return 0.0
+    half = any(t.element_size() == 2 for t in tensors)
+    return (1.5 if not half else 5.0 if ord == 2.0 else 8.5) * U
+
+
+def _check_norm(got, tensors, ord):
+    want = _exact(tensors, ord)
+    assert abs(float(got) - want) <= _tolerance(tensors, ord) * want, (float(got), want)
+
+
+def _check_clip(got, before, max_norm, ord):
+    import torch
+    norm = _exact(before, ord)
+    k = min(1.0, max_norm / (norm + 1e-6))
+    for y, x in zip(got, before):
+        want = x.double() * k
+        fi = torch.finfo(y.dtype)
+        bound = (11 * U + fi.eps / 2 * (1 + 11 * U)) * want.abs() + fi.tiny * fi.eps / 2
+        bad = (y.double() - want).abs() > bound
+        assert not bad.any(), (y.dtype, y[bad][:4], want[bad][:4])
+
+
+SIZES = [[1], [2], [7], [8], [9], [511], [4095], [4097], [100_003], [(3, 5), (1,), (), (0,), (4, 0, 3), (129, 257)],
+         [(1 << 20) + 3, 1, 77_777, (31, 1001)], [(64, 16)] * 150, [5] * 1000, [(1 << 23) + 1, 3]]
+
+
+@pytest.mark.parametrize("ord", ORDS)
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16", "mix"])
+@pytest.mark.parametrize("i", range(len(SIZES)))
+def test_norm_and_clip(cuda, qrc, i, kind, ord):
+    import torch
+    sizes = SIZES[i]
+    kinds = [kind] * len(sizes) if kind != "mix" else [("f32", "bf16", "f16")[j % 3] for j in range(len(sizes))]
+    x = _make(sizes, kinds, seed=i)
+    with qrc.TensorList(x) as tensors:
+        n = tensors.norm(ord)
+        assert n.shape == () and n.dtype == torch.float32
+        _check_norm(n, x, ord)
+        assert torch.equal(n, tensors.norm(ord))                       # the same bits again
+        before = [t.clone() for t in x]
+        max_norm = 0.37 * _exact(x, ord)
+        assert torch.equal(tensors.clip_norm(max_norm, ord), n)
+        _check_clip(x, before, max_norm, ord)
+        # far above the norm: nothing changes
+        kept = [t.clone() for t in x]
+        tensors.clip_norm(1e9, ord)
+        assert all(torch.equal(a, b) for a, b in zip(x, kept))
+
+
+@pytest.mark.parametrize("to", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shift", [0, 1, 3])
+def test_clip_into_other_tensors(cuda, qrc, kind, to, shift):
+    import torch
+    sizes = [1, 9, 4099, (33, 65), 70_001]
+    x = _make(sizes, [kind] * 5, seed=7)
+    # inputs and outputs that start at different distances from 16 bytes
+    x = [torch.cat([t.new_zeros(shift), t.flatten()])[shift:].view(t.shape) for t in x]
+    y = [torch.full((t.numel() + 9,), 5.0, dtype=_types()[to], device=cuda) for t in x]
+    views = [b[2 * shift:2 * shift + t.numel()].view(t.shape) for b, t in zip(y, x)]
+    before = [t.clone() for t in x]
+    for max_norm in (0.5 * _exact(x, 2.0), 1e6):
+        n = qrc.TensorList(x, out=views).clip_norm(max_norm)
+        _check_norm(n, x, 2.0)
+        _check_clip(views, before, max_norm, 2.0)
+        assert all(torch.equal(a, b) for a, b in zip(x, before))
+        for b, t in zip(y, x):                                         # nothing beside the outputs
+            assert (b[:2 * shift] == 5).all() and (b[2 * shift + t.numel():] == 5).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_strided_tensors(cuda, qrc, kind):
+    import torch
+    def views():
+        gen = torch.Generator(device="cuda").manual_seed(3)
+        base = [torch.randn(n, generator=gen, device=cuda).to(_types()[kind]) for n in
+                ((40, 100), (6, 5, 32), (50, 64), (3, 9, 8, 8), (300, 3), (17,), (64, 4096))]
+        return base, [base[0][:, 3:40], base[0][:, 40:], base[1].permute(2, 0, 1), base[2].t()[8:24], base[3][:, ::2, :, 1:7],
+                      base[4][:, 1], base[5][::2], base[6][:, 2048:]]
+    base, v = views()
+    before = [b.clone() for b in base]
+    _, was = views()
+    tensors = qrc.TensorList(v)
+    for ord in ORDS:
+        _check_norm(tensors.norm(ord), v, ord)
+    limit = 0.3 * _exact(v, 2.0)
+    _check_norm(tensors.clip_norm(limit), was, 2.0)
+    _check_clip(v, was, limit, 2.0)
+    inside = [torch.zeros_like(b, dtype=torch.bool) for b in base]       # what no view covers stays
+    for j, view in zip((0, 0, 1, 2, 3, 4, 5, 6), v):
+        torch.as_strided(inside[j], view.shape, view.stride(), view.storage_offset()).fill_(True)
+    for b, c, m in zip(base, before, inside):
+        assert torch.equal(b[~m], c[~m])
+    # into dense outputs, another order of dimensions
+    out = [torch.empty(t.shape, dtype=torch.float32, device=cuda) for t in was]
+    qrc.TensorList(was, out=out).clip_norm(limit)
+    _check_clip(out, was, limit, 2.0)
+
+
+def test_expanded_input(cuda, qrc):
+    import torch
+    x = torch.arange(1.0, 6.0, device=cuda).expand(4, 5)
+    assert float(qrc.TensorList([x]).norm(1.0)) == 60.0
+    out = torch.empty(4, 5, device=cuda)
+    qrc.TensorList([x], out=[out]).clip_norm(6.0, 1.0)
+    _check_clip([out], [x], 6.0, 1.0)
+    with pytest.raises(RuntimeError, match="share memory"):
+        qrc.TensorList([x]).clip_norm(1.0)
+
+
+def test_large_and_small_values(cuda, qrc):
+    import torch
+    # squares leave float's range on both sides, bf16's too
+    for kind in ("f32", "bf16"):
+        for v in (1e30, 3e38, 1e-30, 1e-38):
+            x = [torch.full((1000,), v, device=cuda).to(_types()[kind]), torch.zeros(4096, dtype=_types()[kind], device=cuda)]
+            for ord in ORDS:
+                want = _exact(x, ord)
+                got = float(qrc.TensorList(x).norm(ord))
+                assert got == (math.inf if want > 3.4028235e38 else pytest.approx(want, rel=8.5 * U)), (kind, v, ord)
+    x = [torch.full((5,), 65504.0, dtype=torch.float16, device=cuda), torch.full((64,), 2.0 ** -24, dtype=torch.float16, device=cuda)]
+    for ord in ORDS:
+        _check_norm(qrc.TensorList(x).norm(ord), x, ord)
+    # large and small side by side in one vector of eight
+    y = torch.tensor([1e30, 1e-30, 0, 1, 1e25, -1e25, 3, 4] * 64, device=cuda).to(torch.bfloat16)
+    for ord in ORDS:
+        _check_norm(qrc.TensorList([y]).norm(ord), [y], ord)
+    # float32 subnormals survive
+    s = torch.full((9,), 1e-44, device=cuda)
+    assert float(qrc.TensorList([s]).norm(math.inf)) == float(s[0])
+
+
+@pytest.mark.parametrize("ord", ORDS)
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("at", [0, 5, 4096, 70_000])
+def test_nan_and_infinity(cuda, qrc, kind, ord, at):
+    import torch
+    x = _make([70_001, 33], [kind] * 2)
+    x[0][at] = math.inf
+    t = qrc.TensorList(x)
+    assert float(t.norm(ord)) == math.inf
+    assert float(t.clip_norm(math.inf, ord)) == math.inf                  # no limit: untouched
+    assert float(x[0][at]) == math.inf and torch.isfinite(x[1]).all()
+    x[1][7] = math.nan
+    assert math.isnan(float(t.norm(ord)))
+    y = [torch.empty_like(v) for v in x]
+    assert math.isnan(float(qrc.TensorList(x, out=y).clip_norm(1.0, ord)))
+    assert all(torch.isnan(v).all() for v in y)
+    x[1][7] = 1.0                                                          # infinite norm: the factor is 0
+    qrc.TensorList(x, out=y).clip_norm(1.0, ord)
+    assert torch.isnan(y[0][at]) and (y[1] == 0).all()
+
+
+def test_empty_lists(cuda, qrc):
+    import torch
+    for x in ([], [torch.empty(0, device=cuda)], [torch.empty(3, 0, device=cuda, dtype=torch.bfloat16)] * 2):
+        t = qrc.TensorList(x, device=0)
+        assert float(t.norm()) == 0.0 and float(t.clip_norm(1.0)) == 0.0
+
+
+def test_same_tensor_twice(cuda, qrc):
+    import torch
+    x = torch.ones(100, device=cuda)
+    t = qrc.TensorList([x, x])
+    assert float(t.norm(1.0)) == 200.0
+    with pytest.raises(RuntimeError, match="share memory"):
+        t.clip_norm(1.0)
+    with pytest.raises(RuntimeError, match="share memory"):
+        qrc.TensorList([x[:60], x[50:]]).clip_norm(1.0)
+    assert float(qrc.TensorList([x[:50], x[50:]]).clip_norm(1.0)) == 10.0
+
+
+def test_given_norm_and_outputs(cuda, qrc):
+    import torch
+    x = _make([1000, 33], ["f32", "bf16"])
+    before = [v.clone() for v in x]
+    n = torch.tensor(50.0, device=cuda)
+    assert qrc.TensorList(x).clip_norm(2.0, norm=n) is n and float(n) == 50.0
+    k = 2.0 / (50.0 + 1e-6)
+    for y, w in zip(x, before):
+        assert (y.double() - w.double() * k).abs().max() <= (2 * U + torch.finfo(y.dtype).eps / 2) * w.double().abs().max()
+    out = torch.empty(1, device=cuda)
+    assert qrc.TensorList(before).norm(out=out) is out
+    _check_norm(out, before, 2.0)
+    t = qrc.TensorList(x)
+    for bad in (torch.empty(2, device=cuda), torch.empty(1, device=cuda, dtype=torch.float64), torch.empty(1)):
+        with pytest.raises(RuntimeError, match="one float32"):
+            t.norm(out=bad)
+        with pytest.raises(RuntimeError, match="one float32"):
+            t.clip_norm(1.0, norm=bad)
+    for bad in (-1.0, math.nan):
+        with pytest.raises(RuntimeError, match="max_norm"):
+            t.clip_norm(bad)
+    t.clip_norm(0.0)
+    assert all((v == 0).all() for v in x)
+    t.close()
+    with pytest.raises(RuntimeError, match="closed"):
+        t.norm()
+
+
+def test_two_streams_and_graphs_share_a_list(cuda, qrc):
+    import torch
+    x = _make([3_000_001, 100_003], ["f32", "bf16"])
+    out = [torch.empty(v.shape, device=cuda) for v in x]
+    t = qrc.TensorList(x, out=out)
+    want = {o: float(t.norm(o)) for o in ORDS}
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for s, o in zip(streams, ORDS):
+            got.append((o, t.norm(o, stream=s)))
+        with torch.cuda.stream(streams[0]):
+            got.append((2.0, t.norm(2.0)))
+        got.append((1.0, t.norm(1.0, stream=streams[1].cuda_stream)))
+    torch.cuda.synchronize()
+    assert all(float(v) == want[o] for o, v in got)
+    # two graphs of one list, replayed at the same time on new values
+    graphs = []
+    for o in (1.0, 2.0):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            v = t.norm(o)
+        graphs.append((g, o, v))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        n = t.clip_norm(1.0)
+    t.close()                                               # a captured call carries its own plan
+    x[0].mul_(3.0)
+    want = {o: _exact(x, o) for o in ORDS}
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, (h, _, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                h.replay()
+    g.replay()
+    torch.cuda.synchronize()
+    for _, o, v in graphs:
+        assert abs(float(v) - want[o]) <= 8.5 * U * want[o]
+    _check_clip(out, x, 1.0, 2.0)
+    assert abs(float(n) - want[2.0]) <= 5 * U * want[2.0]
+
+
+def test_follows_the_stream_order(cuda, qrc):
+    """Overlapped launches still wait for what the stream did before."""
+    import torch
+    x = torch.ones(1 << 22, device=cuda)
+    t = qrc.TensorList([x])
+    for i in range(50):
+        x.fill_(float(i + 1))
+        n = t.norm(1.0)
+        t.clip_norm(0.0)
+        m = t.norm(math.inf)
+        x.add_(1.0)
+        assert float(n) == (i + 1) * 2.0 ** 22 and float(m) == 0.0
+
+
+def test_operators(cuda, qrc):
+    import torch
+    import quickruncuda_b200.torch_ops  # noqa: F401
+    x = _make([1000, (33, 7), 12_345], ["f32", "bf16", "f16"])
+    _check_norm(torch.ops.qrc.grad_norm(x), x, 2.0)
+    _check_norm(torch.ops.qrc.grad_norm(x, math.inf), x, math.inf)
+    before = [v.clone() for v in x]
+    versions = [v._version for v in x]
+    _check_norm(torch.ops.qrc.clip_grad_norm_(x, 0.5), before, 2.0)
+    _check_clip(x, before, 0.5, 2.0)
+    assert all(v._version > w for v, w in zip(x, versions))
+
+    def f(a, b):
+        return torch.ops.qrc.clip_grad_norm_([a, b], 0.25), a * 2
+
+    cf = torch.compile(f, backend="aot_eager", fullgraph=True)
+    a, b = x[0].clone(), x[1].clone()
+    n, twice = cf(a, b)
+    _check_norm(n, x[:2], 2.0)
+    _check_clip([a, b], x[:2], 0.25, 2.0)
+    assert torch.equal(twice, a * 2)

@@ -1,0 +1,114 @@
+"""4-bit weights (quickruncuda_b200/weight4.py, qrc_w4_*) without a GPU: what
+is refused before any GPU work, and the shapes of the operators."""
+import ctypes
+
+import pytest
+import torch
+
+import quickruncuda_b200 as q
+import quickruncuda_b200.torch_ops  # noqa: F401  (registers torch.ops.qrc.*)
+from quickruncuda_b200 import _native as nat
+from quickruncuda_b200.weight4 import packed_shape
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+P, S, Z, X, Y, W = (i << 24 for i in range(1, 7))       # addresses far apart, never read
+
+
+def _w4(packed=P, scales=S, zeros=None, n=48, k=300, group=128, type=nat.TYPE_BF16):
+    return ctypes.byref(nat.W4(packed, scales, zeros, n, k, group, type))
+
+
+def test_words(lib):
+    assert lib.qrc_w4_words(0, 5) == 0 and lib.qrc_w4_words(5, 0) == 0
+    assert lib.qrc_w4_words(3, 1) == 48 and lib.qrc_w4_words(3, 128) == 48 and lib.qrc_w4_words(3, 129) == 96
+    for k in (0, 1, 127, 128, 129, 1000):
+        n, words = packed_shape(7, k)
+        assert n * words == lib.qrc_w4_words(7, k)
+
+
+@pytest.mark.parametrize("bad", [dict(group=96), dict(group=16), dict(group=0), dict(group=512), dict(type=nat.TYPE_F32),
+                                 dict(type=7), dict(packed=None), dict(packed=P + 4), dict(scales=None),
+                                 dict(scales=S + 1), dict(n=(1 << 31) + 1), dict(k=(1 << 31) + 1)])
+def test_bad_matrices_are_refused(lib, bad):
+    w = _w4(**bad)
+    k = max(300, bad.get("k", 0))
+    assert lib.qrc_w4_quant(0, X, k, 1, w, None) == nat.QRC_ERR_INVALID
+    assert lib.qrc_w4_pack(0, X, k, w, None) == nat.QRC_ERR_INVALID
+    assert lib.qrc_w4_dequant(0, w, Y, k, nat.TYPE_F32, None) == nat.QRC_ERR_INVALID
+    assert lib.qrc_w4_matvec(0, w, X, 1, k, None, Y, 48, nat.TYPE_F32, None, None) == nat.QRC_ERR_INVALID
+    assert lib.qrc_w4_matvec_workspace(w, X + 2, 1, k) == 0
+
+
+def test_bad_arguments_are_refused(lib):
+    bad = nat.QRC_ERR_INVALID
+    assert lib.qrc_w4_quant(0, X, 300, 1, None, None) == bad
+    assert lib.qrc_w4_quant(0, None, 300, 1, _w4(), None) == bad
+    assert lib.qrc_w4_quant(0, X + 1, 300, 1, _w4(), None) == bad
+    assert lib.qrc_w4_quant(0, X, 299, 1, _w4(), None) == bad                  # rows on top of each other
+    assert lib.qrc_w4_quant(0, X, 300, 0, _w4(), None) == bad                  # zeros to write, none given
+    assert lib.qrc_w4_quant(0, X, 300, 1, _w4(zeros=Z), None) == bad
+    assert lib.qrc_w4_quant(0, S - 600, 300, 1, _w4(), None) == bad            # overwrites its input
+    assert lib.qrc_w4_pack(0, None, 300, _w4(), None) == bad
+    assert lib.qrc_w4_pack(0, X, 299, _w4(), None) == bad
+    assert lib.qrc_w4_dequant(0, _w4(), None, 300, 0, None) == bad
+    assert lib.qrc_w4_dequant(0, _w4(), Y, 300, 3, None) == bad
+    assert lib.qrc_w4_dequant(0, _w4(), Y + 2, 300, 0, None) == bad
+    assert lib.qrc_w4_dequant(0, _w4(), Y, 299, 0, None) == bad
+    assert lib.qrc_w4_dequant(0, _w4(), P + 64, 300, 0, None) == bad
+    ok = dict(device=0, w=_w4(), x=X, m=2, ldx=304, bias=None, y=Y, ldy=48, type=nat.TYPE_BF16, work=None, stream=None)
+    for change in (dict(x=None), dict(y=None), dict(x=X + 1), dict(bias=X + 1), dict(y=Y + 1), dict(ldx=299), dict(ldy=47),
+                   dict(type=nat.TYPE_F16), dict(type=5), dict(y=Y + 2, type=nat.TYPE_F32), dict(m=(1 << 31) + 1),
+                   dict(y=X + 64), dict(y=P), dict(y=S), dict(bias=Y), dict(x=X + 2), dict(x=X, ldx=301),
+                   dict(x=X, ldx=301, work=W + 8)):
+        assert lib.qrc_w4_matvec(*dict(ok, **change).values()) == bad, change
+
+
+def test_workspace(lib):
+    assert lib.qrc_w4_matvec_workspace(_w4(), X, 1, 300) == 0                  # one row, aligned
+    assert lib.qrc_w4_matvec_workspace(_w4(), X, 2, 304) == 0
+    assert lib.qrc_w4_matvec_workspace(_w4(), X, 2, 300) == 2 * 384 * 2
+    assert lib.qrc_w4_matvec_workspace(_w4(), X + 2, 1, 300) == 384 * 2
+    assert lib.qrc_w4_matvec_workspace(_w4(), X + 2, 0, 300) == 0
+
+
+def test_python_refusals():
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        q.quant_w4(torch.ones(4, 4, dtype=torch.bfloat16))
+    with FakeTensorMode():
+        w = torch.empty(48, 300, device="cuda", dtype=torch.bfloat16)
+        for bad, what in ((w.float(), "dtype"), (w[0], "2-D"), (w.t(), "neighbouring"), (w[:, ::2], "neighbouring"),
+                          (w[:1].expand(4, 300), "neighbouring")):
+            with pytest.raises(RuntimeError, match=what):
+                q.quant_w4(bad)
+        with pytest.raises(RuntimeError, match="group"):
+            q.quant_w4(w, group=100)
+        packed = torch.empty(48, 48, device="cuda", dtype=torch.int32)
+        scales = torch.empty(3, 48, device="cuda", dtype=torch.bfloat16)
+        zeros = torch.empty(3, 48, device="cuda", dtype=torch.uint8)
+        for change, what in (((packed.float(), scales, zeros, 300, 128), "packed"), ((packed, scales, zeros, 400, 128), "packed"),
+                             ((packed, scales.float(), zeros, 300, 128), "scales"), ((packed, scales, zeros, 300, 64), "scales"),
+                             ((packed, scales, zeros.int(), 300, 128), "zeros"), ((packed, scales, zeros[:2], 300, 128), "zeros"),
+                             ((packed, torch.empty(48, 3, device="cuda", dtype=torch.bfloat16).t(), None, 300, 128), "contiguous"),
+                             ((packed, scales, zeros, 300, 48), "group"), ((packed, scales, zeros, -1, 128), "k has")):
+            with pytest.raises(RuntimeError, match=what):
+                q.Weight4(*change)
+        with pytest.raises(RuntimeError, match="codes"):
+            q.Weight4.from_codes(packed, scales)
+
+
+def test_operator_shapes():
+    with FakeTensorMode():
+        w = torch.empty(48, 300, device="cuda", dtype=torch.float16)
+        packed, scales, zeros = torch.ops.qrc.quant_w4(w, 64, False)
+        assert packed.shape == (48, 48) and packed.dtype == torch.int32
+        assert scales.shape == (5, 48) == zeros.shape and scales.dtype == torch.float16 and zeros.dtype == torch.uint8
+        assert torch.ops.qrc.quant_w4(w)[2].numel() == 0
+        v = torch.ops.qrc.dequant_w4(packed, scales, zeros, 300, 64)
+        assert v.shape == (48, 300) and v.dtype == torch.float16
+        assert torch.ops.qrc.dequant_w4(packed, scales, None, 300, 64, torch.float32).dtype == torch.float32
+        x = torch.empty(2, 5, 300, device="cuda", dtype=torch.float16)
+        y = torch.ops.qrc.matvec_w4(x, packed, scales, zeros, 64)
+        assert y.shape == (2, 5, 48) and y.dtype == torch.float16
+        assert torch.ops.qrc.matvec_w4(x[0, 0], packed, scales, None, 64, None, torch.float32).dtype == torch.float32
+    with pytest.raises(NotImplementedError):
+        torch.ops.qrc.quant_w4(torch.ones(4, 4, dtype=torch.bfloat16))

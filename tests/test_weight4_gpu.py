@@ -1,0 +1,332 @@
+"""4-bit weights on the GPU: the quantizer and the packed layout code by code,
+the product against the formula in 64 bits.
+
+The product's tolerance: every product and sum is formed in float, so with
+S = sum |value * x| the sum is off by at most (k + groups + 8) * 2^-23 * S
+(one step per addition, whichever way the matrix instruction rounds), and the
+result is rounded once, eps / 2 of it or half the type's smallest number."""
+import math
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def _type(name):
+    import torch
+    return {"bf16": torch.bfloat16, "f16": torch.float16}[name]
+
+
+def _unpack(packed, k):
+    """Codes [n, k] from the layout that qrc_b200.h describes."""
+    import torch
+    n = packed.shape[0]
+    words = packed.view(n, -1, 4, 4).long() & 0xFFFFFFFF                 # [n, block, t, j]
+    codes = torch.empty(n, words.shape[1], 4, 4, 8, dtype=torch.uint8, device=packed.device)   # [n, block, j, t, e]
+    for e in range(8):
+        codes[..., e] = (words >> ((e // 2) * 4 + (e % 2) * 16) & 15).transpose(2, 3).to(torch.uint8)
+    return codes.reshape(n, -1)[:, :k]
+
+
+def _round16(v, kind):
+    """A non-negative double rounded once to a 16-bit type."""
+    import torch
+    bits, low = (8, -125) if kind == torch.bfloat16 else (11, -13)
+    e = torch.frexp(v)[1].clamp(min=low)
+    step = torch.ldexp(torch.ones_like(v), e - bits)
+    return torch.round(v / step) * step
+
+
+def _quant_reference(w, group, symmetric):
+    """(codes, scales, zeros) in 64 bits from the definition."""
+    import torch
+    n, k = w.shape
+    g = -(-k // group)
+    x = torch.zeros(n, g * group, dtype=torch.float64, device=w.device)
+    x[:, :k] = w.double()
+    x = x.view(n, g, group)
+    f = torch.where(torch.isfinite(x), x, torch.zeros_like(x))
+    if symmetric:
+        s, low = _round16(f.abs().amax(2) / 7, w.dtype), 1
+        z = torch.full_like(s, 8)
+    else:
+        s, low = _round16((f.amax(2).clamp(min=0) - f.amin(2).clamp(max=0)) / 15, w.dtype), 0
+        d = torch.where(s > 0, s, torch.ones_like(s))
+        z = torch.where(s > 0, torch.round(-f.amin(2).clamp(max=0) / d), torch.zeros_like(s)).clamp(0, 15)
+    d = torch.where(s > 0, s, torch.ones_like(s))
+    c = (torch.round(x / d[..., None]) + z[..., None]).clamp(low, 15)
+    c = torch.where((s > 0)[..., None] & ~torch.isnan(x), c, z[..., None])
+    return c.view(n, -1)[:, :k].to(torch.uint8), s.t(), z.t().to(torch.uint8)
+
+
+def _check_quant(qrc, w, group, symmetric):
+    import torch
+    w4 = qrc.quant_w4(w, group=group, symmetric=symmetric)
+    codes, scales, zeros = _quant_reference(w, group, symmetric)
+    assert w4.scales.dtype == w.dtype and torch.equal(w4.scales.double(), scales)
+    assert (w4.zeros is None) == symmetric
+    if not symmetric:
+        assert torch.equal(w4.zeros, zeros)
+    got = _unpack(w4.packed, w.shape[1])
+    bad = got != codes
+    assert not bad.any(), (got[bad][:5], codes[bad][:5], w[bad][:5])
+    # the values, exact in float32 and rounded once in 16 bits, within the
+    # types' ranges: with zero 8 and scale max / 7.5, (0 - 8) * scale is
+    # 3.6e38 for the largest bfloat16 weights, more than float32 holds
+    wide = lambda t: t.t().repeat_interleave(group, 1)[:, :w.shape[1]].double()
+    values = (codes.double() - wide(zeros.double())) * wide(scales)
+    lim = torch.finfo(torch.float32).max
+    assert torch.equal(w4.dequant(dtype=torch.float32).double(), values.clamp(-lim, lim))
+    for kind in (torch.bfloat16, torch.float16):
+        lim = torch.finfo(kind).max
+        assert torch.equal(w4.dequant(dtype=kind), values.float().clamp(-lim, lim).to(kind))
+    return w4
+
+
+QUANT_SHAPES = [(1, 1), (1, 7), (3, 8), (5, 31), (2, 33), (16, 128), (17, 129), (9, 255), (4, 256), (7, 257), (33, 1000),
+                (130, 2050), (257, 511)]
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_quant_shapes(cuda, qrc, kind, group, symmetric):
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(group)
+    for n, k in QUANT_SHAPES:
+        w = torch.randn(n, k, generator=gen, device=cuda).mul_(0.05).to(_type(kind))
+        _check_quant(qrc, w, group, symmetric)
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_quant_borders_and_special_values(cuda, qrc, kind, symmetric):
+    import torch
+    t = _type(kind)
+    fi = torch.finfo(t)
+    rows = []
+    rows.append(torch.arange(-64, 64, device=cuda) / 16.0)                     # many quotients on k + 1/2
+    rows.append(torch.arange(0, 128, device=cuda) / 128.0 * 7)                 # no negative number
+    rows.append(-torch.arange(0, 128, device=cuda) / 32.0)
+    rows.append(torch.zeros(128, device=cuda))
+    rows.append(torch.full((128,), 0.3, device=cuda))
+    rows.append(torch.linspace(-fi.max, fi.max, 128, dtype=torch.float64, device=cuda).clamp(-fi.max, fi.max))
+    rows.append(torch.linspace(-1, 1, 128, device=cuda) * fi.tiny * fi.eps * 40)
+    rows.append(torch.linspace(-1, 1, 128, device=cuda) * fi.tiny * fi.eps * 3)
+    rows.append(torch.linspace(-1, 1, 128, device=cuda) * fi.tiny)
+    odd = torch.randn(128, device=cuda, generator=torch.Generator(device="cuda").manual_seed(1))
+    rows.append(odd.clone().index_fill_(0, torch.tensor([3, 40, 90], device=cuda), math.nan))
+    rows.append(odd.clone().index_fill_(0, torch.tensor([5, 64], device=cuda), math.inf))
+    rows.append(odd.clone().index_fill_(0, torch.tensor([5, 64], device=cuda), -math.inf))
+    rows.append(torch.full((128,), math.nan, device=cuda))
+    rows.append(torch.full((128,), math.inf, device=cuda))
+    rows.append(torch.full((128,), -0.0, device=cuda))
+    w = torch.stack([r.double() for r in rows]).to(t)
+    for group in (32, 128):
+        w4 = _check_quant(qrc, w, group, symmetric)
+        assert torch.isfinite(w4.dequant()).all()
+    # wide spread: the difference max - min is not a float
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    spread = torch.randn(4096, 64, generator=gen, device=cuda) * torch.exp2(
+        torch.randint(-12 if kind == "f16" else -60, 4, (4096, 64), generator=gen, device=cuda).float())
+    _check_quant(qrc, spread.to(t), 32, symmetric)
+
+
+def test_quant_of_views(cuda, qrc):
+    import torch
+    w = torch.randn(40, 600, device=cuda).to(torch.bfloat16)
+    for v in (w[:, :512], w[:, 1:300], w[3:, 8:], w[::2], w[5:6, 7:9]):
+        _check_quant(qrc, v, 64, False)
+    out = torch.full((40, 700), 9.0, device=cuda)
+    w4 = qrc.quant_w4(w)
+    for sub in (out[:, :600], out[:, 100:], out[:, 37:637]):
+        out.fill_(9.0)
+        assert torch.equal(w4.dequant(out=sub), w4.dequant(dtype=torch.float32))
+        assert int((out == 9.0).sum()) >= 40 * 100
+
+
+def _case(cuda, n, k, kind, group, symmetric, seed=0, spread=True):
+    import torch
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    codes = torch.randint(0, 16, (n, k), generator=gen, device=cuda, dtype=torch.uint8)
+    g = -(-k // group)
+    scales = torch.rand(g, n, generator=gen, device=cuda) * 0.01 + 0.001
+    if spread:
+        scales = scales * torch.exp2(torch.randint(-3, 4, (g, n), generator=gen, device=cuda).float())
+    scales = scales.to(_type(kind))
+    zeros = None if symmetric else torch.randint(0, 16, (g, n), generator=gen, device=cuda, dtype=torch.uint8)
+    return codes, scales, zeros, gen
+
+
+def _values(codes, scales, zeros, group):
+    import torch
+    wide = lambda t: t.t().repeat_interleave(group, 1)[:, :codes.shape[1]].double()
+    z = torch.full_like(scales, 8).double() if zeros is None else zeros.double()
+    return (codes.double() - wide(z)) * wide(scales)
+
+
+def _check_product(y, x, values, bias, group):
+    import torch
+    k = values.shape[1]
+    x2 = x.reshape(-1, k).double()
+    want = x2 @ values.t() + (0 if bias is None else bias.double())
+    s = x2.abs() @ values.abs().t() + (0 if bias is None else bias.double().abs())
+    fi = torch.finfo(y.dtype)
+    bound = (k + k / group + 8) * 2.0 ** -23 * s * (1 + fi.eps) + fi.eps / 2 * want.abs() + fi.tiny * fi.eps / 2
+    got = y.reshape(want.shape).double()
+    bad = (got - want).abs() > bound
+    assert not bad.any(), (got[bad][:4], want[bad][:4], bound[bad][:4])
+
+
+MATVEC_SHAPES = [(1, 1), (1, 130), (15, 31), (16, 32), (17, 33), (48, 127), (33, 128), (100, 129), (7, 1000), (130, 264),
+                 (64, 4096), (5, 20_001), (1025, 640)]
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_matvec_shapes(cuda, qrc, kind, group, symmetric):
+    import torch
+    for i, (n, k) in enumerate(MATVEC_SHAPES):
+        codes, scales, zeros, gen = _case(cuda, n, k, kind, group, symmetric, seed=i)
+        w4 = qrc.Weight4.from_codes(codes, scales, zeros, group=group)
+        assert torch.equal(_unpack(w4.packed, k), codes)
+        values = _values(codes, scales, zeros, group)
+        for m in (1, 2, 3, 7, 8, 9, 16, 17, 32, 33, 70) if i % 4 == 0 else (1, 5, 13, 31):
+            x = torch.randn(m, k, generator=gen, device=cuda).to(_type(kind))
+            bias = torch.randn(n, generator=gen, device=cuda).to(_type(kind)) if m % 2 else None
+            y = w4.matvec(x, bias=bias)
+            assert y.shape == (m, n) and y.dtype == _type(kind)
+            _check_product(y, x, values, bias, group)
+            f = w4.matvec(x, bias=bias, out_dtype=torch.float32)
+            assert f.dtype == torch.float32
+            _check_product(f, x, values, bias, group)
+            assert torch.equal(f, w4.matvec(x, bias=bias, out_dtype=torch.float32))      # the same bits again
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_matvec_of_views(cuda, qrc, kind):
+    import torch
+    n, k, group = 70, 400, 64
+    codes, scales, zeros, gen = _case(cuda, n, k, kind, group, False)
+    wide = torch.full((n, k + 5), 255, dtype=torch.uint8, device=cuda)     # codes in a wider buffer, other high bits
+    wide[:, 2:2 + k] = codes + 48
+    w4 = qrc.Weight4.from_codes(wide[:, 2:2 + k], scales, zeros, group=group)
+    values = _values(codes, scales, zeros, group)
+    buf = torch.randn(12, 2 * k + 16, generator=gen, device=cuda).to(_type(kind))
+    bias = torch.randn(n + 1, generator=gen, device=cuda).to(_type(kind))[1:]
+    for x in (buf[:, :k], buf[:, 8:8 + k], buf[:, 1:1 + k], buf[::3, 16:16 + k], buf[2, :k], buf[2, 3:3 + k],
+              buf[:, :k].view(3, 4, k), buf[:, 3:3 + k].view(3, 2, 2, k), buf[:1, 5:5 + k]):
+        out = torch.full(x.shape[:-1] + (n + 3,), 77.0, device=cuda)
+        if x.dim() == 2:
+            assert w4.matvec(x, bias=bias, out=out[:, 2:2 + n]) is not None
+            _check_product(out[:, 2:2 + n], x, values, bias, group)
+            assert (out[:, :2] == 77).all() and (out[:, 2 + n:] == 77).all()
+        y = w4.matvec(x, bias=bias)
+        assert y.shape == x.shape[:-1] + (n,)
+        _check_product(y, x, values, bias, group)
+    with pytest.raises(RuntimeError, match="one distance"):               # rows at two distances
+        w4.matvec(buf[:, :2 * k].view(12, 2, k), bias=bias)
+
+
+def test_matvec_edges(cuda, qrc):
+    import torch
+    codes, scales, zeros, gen = _case(cuda, 40, 300, "bf16", 128, True)
+    w4 = qrc.Weight4.from_codes(codes, scales, zeros)
+    bf = torch.bfloat16
+    assert w4.matvec(torch.empty(0, 300, dtype=bf, device=cuda)).shape == (0, 40)
+    none = qrc.Weight4.from_codes(codes[:, :0], scales[:0], None)
+    bias = torch.randn(40, device=cuda).to(bf)
+    assert torch.equal(none.matvec(torch.empty(3, 0, dtype=bf, device=cuda), bias=bias), bias.expand(3, 40))
+    assert none.dequant().shape == (40, 0)
+    flat = qrc.Weight4.from_codes(codes[:0], scales[:, :0], None)
+    assert flat.matvec(torch.ones(3, 300, dtype=bf, device=cuda)).shape == (3, 0)
+    assert qrc.quant_w4(torch.empty(0, 5, dtype=bf, device=cuda)).dequant().shape == (0, 5)
+    assert qrc.quant_w4(torch.empty(5, 0, dtype=bf, device=cuda)).scales.shape == (0, 5)
+    # NaN and infinity reach their own row alone
+    x = torch.randn(5, 300, generator=gen, device=cuda).to(bf)
+    clean = w4.matvec(x)
+    x[1, 299], x[3, 0] = math.nan, math.inf
+    y = w4.matvec(x)
+    assert torch.isnan(y[1]).all() and not torch.isfinite(y[3]).any()
+    assert torch.equal(y[[0, 2, 4]], clean[[0, 2, 4]])
+    # what stands behind column k of a wider buffer does not count
+    wide = torch.full((5, 304), math.nan, dtype=bf, device=cuda)
+    wide[:, :300] = torch.randn(5, 300, device=cuda).to(bf)
+    assert torch.equal(w4.matvec(wide[:, :300]), w4.matvec(wide[:, :300].contiguous()))
+
+
+def test_matvec_refusals(cuda, qrc):
+    import torch
+    codes, scales, zeros, _ = _case(cuda, 40, 300, "bf16", 128, True)
+    w4 = qrc.Weight4.from_codes(codes, scales, zeros)
+    x = torch.ones(2, 300, dtype=torch.bfloat16, device=cuda)
+    for args, what in ((dict(x=x.half()), "dtype"), (dict(x=x[:, :299]), "needs"), (dict(x=x.cpu()), "CUDA"),
+                       (dict(x=x.t().contiguous().t()), "neighbouring"), (dict(x=x[:1].expand(2, 300)), "neighbouring"),
+                       (dict(x=x, bias=x[0, :40].float()), "dtype"), (dict(x=x, bias=x[0, :39]), "shape"),
+                       (dict(x=x, bias=x[0, :80:2]), "bias"), (dict(x=x, out_dtype=torch.float16), "float32"),
+                       (dict(x=x, out=torch.empty(2, 39, dtype=x.dtype, device=cuda)), "shape"),
+                       (dict(x=x, out=torch.empty(2, 40, device=cuda), out_dtype=torch.bfloat16), "dtype"),
+                       (dict(x=torch.ones((), dtype=x.dtype, device=cuda)), "shape")):
+        with pytest.raises(RuntimeError, match=what):
+            w4.matvec(**args)
+    big = torch.ones(4, 300, dtype=torch.bfloat16, device=cuda)
+    with pytest.raises(qrc.QrcError):
+        w4.matvec(big[:2], out=big[:2, :40])                        # would overwrite what it reads
+    with pytest.raises(RuntimeError, match="dequant"):
+        w4.dequant(dtype=torch.float64)
+
+
+def test_streams_and_graphs(cuda, qrc):
+    import torch
+    codes, scales, zeros, gen = _case(cuda, 500, 1003, "f16", 32, False)
+    values = _values(codes, scales, zeros, 32)
+    x = torch.randn(3, 1003, generator=gen, device=cuda).half()           # odd rows: laid out on the way
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    w4 = qrc.Weight4.from_codes(codes, scales, zeros, group=32, stream=s)
+    y = [w4.matvec(x, stream=s) for _ in range(10)]
+    s.synchronize()
+    want = w4.matvec(x)
+    _check_product(want, x, values, None, 32)
+    assert all(torch.equal(v, want) for v in y)
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = w4.matvec(x)
+        graphs.append((g, out))
+    x.mul_(-2.0)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        graphs[0][0].replay()
+    graphs[1][0].replay()
+    torch.cuda.synchronize()
+    for _, out in graphs:
+        assert torch.equal(out, want * -2)
+    # quantize, product and dequantize in a row, overlapped launches in order
+    w = torch.randn(500, 1003, device=cuda).half()
+    for i in range(10):
+        w.add_(0.25)
+        a = qrc.quant_w4(w, group=32, symmetric=False)
+        b = a.matvec(x)
+        _check_product(b, x, a.dequant(dtype=torch.float32).double(), None, 32)
+
+
+def test_operators(cuda, qrc):
+    import torch
+    import quickruncuda_b200.torch_ops  # noqa: F401
+    w = torch.randn(48, 300, device=cuda).to(torch.bfloat16)
+    x = torch.randn(2, 3, 300, device=cuda).to(torch.bfloat16)
+    for symmetric in (True, False):
+        a = qrc.quant_w4(w, group=64, symmetric=symmetric)
+
+        def f(w, x):
+            packed, scales, zeros = torch.ops.qrc.quant_w4(w * 1.0, 64, symmetric)
+            return (packed, torch.ops.qrc.dequant_w4(packed, scales, zeros, 300, 64),
+                    torch.ops.qrc.matvec_w4(x, packed, scales, zeros, 64, None, torch.float32))
+
+        for g in (f, torch.compile(f, backend="aot_eager", fullgraph=True)):
+            packed, values, y = g(w, x)
+            assert torch.equal(packed, a.packed) and torch.equal(values, a.dequant())
+            assert torch.equal(y, a.matvec(x, out_dtype=torch.float32))
