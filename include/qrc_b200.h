@@ -350,13 +350,15 @@ int qrc_list_clip(const qrc_list* list, int norm, double max_norm, const float* 
  *
  *   value[n][k] = (code[n][k] - zero[g][n]) * scale[g][n],   g = k / group
  *
- * d_packed holds n rows of ceil(k / 128) blocks of 16 words (16-byte
- * aligned).  Word 4*t + j of a block (t, j < 4) holds columns
- * 32*j + 8*t + 0..7 of the block's 128: column 2*i in bits 4*i..4*i+3, column
- * 2*i + 1 in bits 16 + 4*i..19 + 4*i.  Codes behind column k may be anything.
+ * d_packed holds ceil(n / 16) x ceil(k / 128) tiles of 16 rows by 128 columns,
+ * 256 words each (16-byte aligned), the tiles of 16 rows one after another.
+ * Row r of a tile is its words 16*r .. 16*r + 15; word 4*t + j of a row
+ * (t, j < 4) holds the tile's columns 32*j + 8*t + 0..7, column e of them in
+ * four bits from bit 3 + 4*(e / 2) + 16*(e % 2), counted modulo 32.  What
+ * stands behind row n and column k may be anything.
  * d_scales is [ceil(k / group)][n] of `type`; d_zeros is [ceil(k / group)][n]
  * whole numbers 0..15, or NULL: every zero is 8.  Rows and columns go up to
- * 2^31.  The memory is the caller's; an output that overlaps an input is refused
+ * 2^31 - 1.  The memory is the caller's; an output that overlaps an input is refused
  * (QRC_ERR_INVALID). */
 typedef struct qrc_w4 {
     uint32_t* d_packed;
@@ -397,12 +399,10 @@ int qrc_w4_dequant(int device, const qrc_w4* w, void* d_out, uint64_t ld, int ou
  * formed in float, per group before its scale (so |x| * 15 * group has to
  * stay in float's range), in an order that depends on the sizes alone; the
  * result is rounded once.  Made for a few rows (a decode step); any m >= 0
- * works.  Rows of d_x that do not start on 16
- * bytes need a workspace (16-byte aligned, qrc_w4_matvec_workspace bytes; 0
- * when none is needed).  Asynchronous. */
+ * works.  An infinite or NaN activation gives NaN.  If a bounded wait inside
+ * the kernel gives up (about 1 s), the results are NaN.  Asynchronous. */
 int qrc_w4_matvec(int device, const qrc_w4* w, const void* d_x, uint64_t m, uint64_t ldx, const void* d_bias,
-                  void* d_y, uint64_t ldy, int y_type, void* d_work, void* stream);
-size_t qrc_w4_matvec_workspace(const qrc_w4* w, const void* d_x, uint64_t m, uint64_t ldx);
+                  void* d_y, uint64_t ldy, int y_type, void* stream);
 
 /* Synthetic inputs generated on the device; element i of the stream is a pure
  * function of (seed, offset + i), so shards of one stream can be generated

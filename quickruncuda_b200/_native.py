@@ -114,8 +114,7 @@ SIGNATURES = [
     ("qrc_w4_pack", c_int, [c_int, c_void_p, c_u64, ctypes.POINTER(W4), c_void_p]),
     ("qrc_w4_dequant", c_int, [c_int, ctypes.POINTER(W4), c_void_p, c_u64, c_int, c_void_p]),
     ("qrc_w4_matvec", c_int, [c_int, ctypes.POINTER(W4), c_void_p, c_u64, c_u64, c_void_p, c_void_p, c_u64, c_int,
-                              c_void_p, c_void_p]),
-    ("qrc_w4_matvec_workspace", c_size, [ctypes.POINTER(W4), c_void_p, c_u64, c_u64]),
+                              c_void_p]),
     ("qrc_fill_uniform_f32", c_int, [c_void_p, c_size, c_u64, c_u64, c_void_p]),
     ("qrc_fill_normal_f32", c_int, [c_void_p, c_size, c_u64, c_u64, c_float, c_void_p]),
     ("qrc_fill_normal_bf16", c_int, [c_void_p, c_size, c_u64, c_u64, c_float, c_void_p]),

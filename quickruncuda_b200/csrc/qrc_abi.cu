@@ -826,24 +826,6 @@ static size_t launch_smem(const qrc_ctx* c) {
     return c->bulk_slots ? (size_t)(c->threads / 32) * c->bulk_slots * qrc::kSlotStride : 0;
 }
 
-// Raises a kernel's dynamic shared memory limit on the current device to at
-// least `smem` (launches above 48 KiB need it).  The attribute is per device,
-// so what was granted is remembered per (kernel, device); thread-safe.
-static cudaError_t grant_smem(const void* kernel, size_t smem) {
-    if (smem <= 48 * 1024) return cudaSuccess;
-    static std::mutex mu;
-    static std::map<std::pair<const void*, int>, size_t> granted;
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    std::lock_guard<std::mutex> lock(mu);
-    size_t& g = granted[{kernel, dev}];
-    if (smem <= g) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) g = smem;
-    return e;
-}
-
 template <int T>
 static cudaError_t allow_smem(size_t smem) {
     cudaError_t e = grant_smem((const void*)qrc_k_absmax_f32<T>, smem);

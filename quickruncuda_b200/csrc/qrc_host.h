@@ -3,6 +3,9 @@
 
 #include <cuda_runtime.h>
 #include <cstdint>
+#include <map>
+#include <mutex>
+#include <utility>
 
 #define QRC_API extern "C" __attribute__((visibility("default")))
 
@@ -64,4 +67,22 @@ inline cudaError_t launch_overlapped(void (*kernel)(KArgs...), dim3 grid, int bl
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Raises a kernel's dynamic shared memory limit on the current device to at
+// least `smem` (launches above 48 KiB need it).  The attribute is per device,
+// so what was granted is remembered per (kernel, device); thread-safe.
+inline cudaError_t grant_smem(const void* kernel, size_t smem) {
+    if (smem <= 48 * 1024) return cudaSuccess;
+    static std::mutex mu;
+    static std::map<std::pair<const void*, int>, size_t> granted;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    std::lock_guard<std::mutex> lock(mu);
+    size_t& g = granted[{kernel, dev}];
+    if (smem <= g) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) g = smem;
+    return e;
 }

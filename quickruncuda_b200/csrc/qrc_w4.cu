@@ -5,12 +5,20 @@
 //   value[n][k] = (code[n][k] - zero[g][n]) * scale[g][n],  g = k / group
 //   y[m][n]     = sum_g scale[g][n] * sum_{k in g} (code - zero) * x[m][k]  (+ bias[n])
 //
-// Packed layout.  A row is padded to whole blocks of 128 columns, 64 bytes
-// each.  Word 4*t + j of a block (t, j < 4) holds columns 32*j + 8*t + 0..7:
-// column 2*i in bits 4*i, column 2*i + 1 in bits 16 + 4*i.  A lane of the
-// product's matrix instruction then reads its 16 bytes of a row with one
-// load, each (word >> 4*i) & 0x000f000f is a pair of neighbouring columns,
-// and the four lanes of a row share one group of 32 columns at a time.
+// Packed layout.  Tiles of 16 rows by 128 columns, 1 KiB each, the tiles of a
+// row of tiles one after another: a warp of the product streams contiguous
+// memory, 512 bytes per load.  Row r of a tile is its words 16*r .. 16*r + 15;
+// word 4*t + j of a row (t, j < 4) holds columns 32*j + 8*t + 0..7, so the four
+// lanes that share a row in a matrix instruction read it with one load each
+// and work on one group of 32 columns at a time.  Column e of a word sits at
+// bit 3 + 4*(e / 2) + 16*(e % 2), modulo 32: a rotation by 0, 4, 8 or 12 and
+// one mask bring two neighbouring columns to bits 3..6 of both halves.  There
+// they are the upper mantissa bits of a bfloat16 (16 + code with the exponent
+// of 16) or an fp16 subnormal (code * 2^-21).  Read as bytes, the same word
+// holds four codes times 8 under the mask 0x78787878, and the other four
+// after a rotation by 4.
+#define QRC_NO_PLUGIN_ABI
+#include "side_aware_b200.cu"
 #include "qrc_host.h"
 #include "../../include/qrc_b200.h"
 
@@ -21,55 +29,74 @@
 
 namespace {
 
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+constexpr uint32_t kCodeMask = 0x00780078u;
 
-// What the kernels need of the two 16-bit types.  kOne | code is the value
-// kBias + code: the codes are the last bits of the mantissa.
+// What the kernels need of the two 16-bit types.  (bits & kCodeMask) | kOne is
+// the pair of values (kBias + code) * kUnit.
 template <class T> struct Half;
 template <> struct Half<__nv_bfloat16> {
-    static constexpr uint32_t kOne = 0x43004300u;         // 128
+    using Pair = __nv_bfloat162;
+    static constexpr uint32_t kOne = 0x41804180u;
+    static constexpr float kBias = 16.0f, kUnit = 1.0f;
     static constexpr float kMax = 3.3895313892515355e38f;
-    static __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-    static __device__ __forceinline__ __nv_bfloat16 round(float x) { return __float2bfloat16_rn(x); }
     static __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
-        const __nv_bfloat162 r = __hsub2(reinterpret_cast<__nv_bfloat162&>(a), reinterpret_cast<__nv_bfloat162&>(b));
+        const Pair r = __hsub2(reinterpret_cast<Pair&>(a), reinterpret_cast<Pair&>(b));
         return reinterpret_cast<const uint32_t&>(r);
     }
-    static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                               uint32_t b0, uint32_t b1) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+    static __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+    static __device__ __forceinline__ __nv_bfloat16 round(float x) { return __float2bfloat16_rn(x); }
+    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
                      "{%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
 };
 template <> struct Half<__half> {
-    static constexpr uint32_t kOne = 0x64006400u;         // 1024
+    using Pair = __half2;
+    static constexpr uint32_t kOne = 0u;
+    static constexpr float kBias = 0.0f, kUnit = 0x1p-21f;
     static constexpr float kMax = 65504.0f;
-    static __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-    static __device__ __forceinline__ __half round(float x) { return __float2half_rn(x); }
     static __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
-        const __half2 r = __hsub2(reinterpret_cast<__half2&>(a), reinterpret_cast<__half2&>(b));
+        const Pair r = __hsub2(reinterpret_cast<Pair&>(a), reinterpret_cast<Pair&>(b));
         return reinterpret_cast<const uint32_t&>(r);
     }
-    static __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                               uint32_t b0, uint32_t b1) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+    static __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+    static __device__ __forceinline__ __half round(float x) { return __float2half_rn(x); }
+    static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
                      "{%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                     : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
 };
 
-// Column of the first code of word `word` of a row.
-__device__ __forceinline__ uint64_t word_column(uint64_t word) {
-    const uint32_t i = (uint32_t)word & 15;
-    return (word >> 4) * 128 + (i & 3) * 32 + (i >> 2) * 8;
+template <class T> __device__ __forceinline__ T from_bits(uint32_t b) {
+    const uint16_t h = (uint16_t)b;
+    return reinterpret_cast<const T&>(h);
 }
 
+__device__ __forceinline__ uint32_t rotate_right(uint32_t w, int by) { return __funnelshift_r(w, w, by); }
+
+// Columns 2*i and 2*i + 1 of a word as a pair of T: (kBias + code) * kUnit.
+template <class T> __device__ __forceinline__ uint32_t code_pair(uint32_t word, int i) {
+    return (rotate_right(word, 4 * i) & kCodeMask) | Half<T>::kOne;
+}
+
+// Column, within its tile, of the first code of word `i` of a row.
+__device__ __forceinline__ uint32_t word_column(uint32_t i) { return (i & 3) * 32 + (i >> 2) * 8; }
+
 // Bit position of code e (0..7) in its word.
-__device__ __forceinline__ int code_shift(int e) { return (e >> 1) * 4 + (e & 1) * 16; }
+__device__ __forceinline__ int code_shift(int e) { return (3 + (e >> 1) * 4 + (e & 1) * 16) & 31; }
+
+__device__ __forceinline__ uint32_t place_code(uint32_t code, int e) {
+    return __funnelshift_l(code, code, code_shift(e));
+}
+
+// Word `i` of row `row`, tile column `tile`, of a matrix `tiles` tiles wide.
+__device__ __forceinline__ uint64_t word_at(uint64_t row, uint64_t tile, uint64_t tiles, uint32_t i) {
+    return ((row >> 4) * tiles + tile) * 256 + (row & 15) * 16 + i;
+}
 
 // -- quantize --------------------------------------------------------------------
 
@@ -96,19 +123,19 @@ template <class T>
 __global__ void __launch_bounds__(256)
 qrc_k_w4_quant(const T* w, uint64_t ld, uint64_t n, uint64_t k, int group, int symmetric, int vec,
                uint32_t* packed, T* scales, uint8_t* zeros) {
-    wait_for_previous();
-    let_next_start();
+    qrc::griddep_wait();
+    qrc::griddep_launch_dependents();
     const int lane = threadIdx.x & 31;
-    const uint64_t blocks128 = (k + 127) / 128, windows = (k + 255) / 256;
-    const uint64_t tasks = n * windows;
+    const uint64_t tiles = (k + 127) / 128, windows = (k + 255) / 256;
+    const uint64_t tasks = (n + 15) / 16 * 16 * windows;
     for (uint64_t task = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); task < tasks; task += (uint64_t)gridDim.x * 8) {
         const uint64_t row = task / windows, k0 = (task - row * windows) * 256 + lane * 8;
         const T* p = w + row * ld + k0;
         T v[8];
-        if (vec && k0 + 8 <= k) *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(p);
+        if (vec && row < n && k0 + 8 <= k) *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(p);
         else {
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = k0 + i < k ? p[i] : Half<T>::round(0.0f);
+            for (int i = 0; i < 8; i++) v[i] = row < n && k0 + i < k ? p[i] : Half<T>::round(0.0f);
         }
         float x[8], most = 0.0f, least = 0.0f;
 #pragma unroll
@@ -134,12 +161,12 @@ qrc_k_w4_quant(const T* w, uint64_t ld, uint64_t n, uint64_t k, int group, int s
         for (int i = 0; i < 8; i++) {
             float c = z;
             if (s > 0.0f && x[i] == x[i]) c = fminf(fmaxf(rintf(__fdiv_rn(x[i], s)) + z, low), 15.0f);
-            word |= (uint32_t)c << code_shift(i);
+            word |= place_code((uint32_t)c, i);
         }
-        const uint64_t b = k0 >> 7;
+        const uint64_t tile = k0 >> 7;
         const uint32_t i16 = lane & 15;
-        if (b < blocks128) packed[(row * blocks128 + b) * 16 + (i16 & 3) * 4 + (i16 >> 2)] = word;
-        if (k0 % group == 0 && k0 < k) {
+        if (tile < tiles) packed[word_at(row, tile, tiles, (i16 & 3) * 4 + (i16 >> 2))] = word;
+        if (k0 % group == 0 && k0 < k && row < n) {
             scales[k0 / group * n + row] = Half<T>::round(s);
             if (!symmetric) zeros[k0 / group * n + row] = (uint8_t)z;
         }
@@ -150,15 +177,16 @@ qrc_k_w4_quant(const T* w, uint64_t ld, uint64_t n, uint64_t k, int group, int s
 
 __global__ void __launch_bounds__(256)
 qrc_k_w4_pack(const uint8_t* codes, uint64_t ld, uint64_t n, uint64_t k, uint32_t* packed) {
-    wait_for_previous();
-    let_next_start();
-    const uint64_t words = (k + 127) / 128 * 16, total = n * words;
+    qrc::griddep_wait();
+    qrc::griddep_launch_dependents();
+    const uint64_t tiles = (k + 127) / 128, total = (n + 15) / 16 * tiles * 256;
     for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) {
-        const uint64_t row = i / words, col = word_column(i - row * words);
+        const uint64_t tile = i >> 8, above = tile / tiles;
+        const uint64_t row = above * 16 + ((i >> 4) & 15), col = (tile - above * tiles) * 128 + word_column(i & 15);
         uint32_t word = 0;
 #pragma unroll
         for (int e = 0; e < 8; e++)
-            if (col + e < k) word |= (uint32_t)(codes[row * ld + col + e] & 15) << code_shift(e);
+            if (row < n && col + e < k) word |= place_code(codes[row * ld + col + e] & 15u, e);
         packed[i] = word;
     }
 }
@@ -182,19 +210,20 @@ template <class T, class TO>
 __global__ void __launch_bounds__(256)
 qrc_k_w4_dequant(const uint32_t* packed, const T* scales, const uint8_t* zeros, uint64_t n, uint64_t k, int group,
                  TO* out, uint64_t ld, int vec) {
-    wait_for_previous();
-    let_next_start();
-    const uint64_t words = (k + 127) / 128 * 16, total = n * words;
+    qrc::griddep_wait();
+    qrc::griddep_launch_dependents();
+    const uint64_t tiles = (k + 127) / 128, total = (n + 15) / 16 * tiles * 256;
     for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) {
-        const uint64_t row = i / words, col = word_column(i - row * words);
-        if (col >= k) continue;
+        const uint64_t tile = i >> 8, above = tile / tiles;
+        const uint64_t row = above * 16 + ((i >> 4) & 15), col = (tile - above * tiles) * 128 + word_column(i & 15);
+        if (row >= n || col >= k) continue;
         const uint32_t word = packed[i];
         const uint64_t at = col / group * n + row;
         const float s = Half<T>::to_float(scales[at]);
         const float z = zeros ? (float)zeros[at] : 8.0f;
         __align__(16) TO v[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = round_to<TO>(((float)((word >> code_shift(e)) & 15u) - z) * s);
+        for (int e = 0; e < 8; e++) v[e] = round_to<TO>(((float)(rotate_right(word, code_shift(e)) & 15u) - z) * s);
         TO* q = out + row * ld + col;
         if (vec && col + 8 <= k) {
 #pragma unroll
@@ -208,20 +237,6 @@ qrc_k_w4_dequant(const uint32_t* packed, const T* scales, const uint8_t* zeros, 
 
 // -- product -----------------------------------------------------------------------
 
-// Activations whose rows do not start on 16 bytes, copied into rows of whole
-// 128-column blocks, zero behind column k.
-template <class T>
-__global__ void __launch_bounds__(256)
-qrc_k_w4_lay_out(const T* x, uint64_t ldx, uint64_t m, uint64_t k, T* to) {
-    wait_for_previous();
-    let_next_start();
-    const uint64_t width = (k + 127) / 128 * 128, total = m * width;
-    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) {
-        const uint64_t row = i / width, col = i - row * width;
-        to[i] = col < k ? x[row * ldx + col] : Half<T>::round(0.0f);
-    }
-}
-
 struct W4 {
     const uint32_t* packed;
     const void* scales;
@@ -230,94 +245,451 @@ struct W4 {
     int group_log2;
 };
 
-constexpr int kWarps = 8;
-
-// Eight activations from column k0 of a row, zero behind column k.
-template <class T>
-__device__ __forceinline__ uint4 load_x(const T* row, uint64_t k0, uint64_t k) {
-    if (k0 + 8 <= k) return *reinterpret_cast<const uint4*>(row + k0);
-    __align__(16) T v[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = k0 + i < k ? row[k0 + i] : Half<T>::round(0.0f);
-    return *reinterpret_cast<const uint4*>(v);
+// (c0, c1) += a * (b0, b1): one instruction for both where `a` serves several
+// pairs, as it has to be copied into a pair of its own.
+template <int PAIRS> __device__ __forceinline__ void add_scaled(float& c0, float& c1, float a, float b0, float b1) {
+    if (PAIRS == 1) {
+        c0 = fmaf(a, b0, c0);
+        c1 = fmaf(a, b1, c1);
+        return;
+    }
+    asm("{ .reg .b64 x, y, z;\n\t"
+        "mov.b64 x, {%2, %2};\n\t"
+        "mov.b64 y, {%3, %4};\n\t"
+        "mov.b64 z, {%0, %1};\n\t"
+        "fma.rn.f32x2 z, x, y, z;\n\t"
+        "mov.b64 {%0, %1}, z; }"
+        : "+f"(c0), "+f"(c1) : "f"(a), "f"(b0), "f"(b1));
 }
 
-// A block computes 16 rows of weights times 8 * NT rows of activations; its
-// warps take the 128-column blocks in turn and add their sums in a fixed
-// order.  The codes, as differences code - zero, are exact in 16 bits, and
-// the matrix instruction multiplies and adds them in 32; the scale of a group
-// (128 / SUB columns, or a multiple of 128 with SUB = 1) multiplies its sum.
-template <class T, int NT, int SUB>
-__global__ void __launch_bounds__(kWarps * 32)
-qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t kx, uint64_t m, const T* bias, void* y, uint64_t ldy,
-                int y_float) {
-    wait_for_previous();
-    let_next_start();
-    __shared__ float s_sum[kWarps][16][8 * NT];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const uint64_t n0 = (uint64_t)blockIdx.x * 16, m0 = (uint64_t)blockIdx.y * 8 * NT;
-    const uint64_t blocks = (w.k + 127) / 128, groups = (w.k + (1ull << w.group_log2) - 1) >> w.group_log2;
-    // Rows behind the last one repeat it; their sums are not stored.
-    const uint64_t ra = min(n0 + g, w.n - 1), rb = min(n0 + g + 8, w.n - 1);
-    const uint4* pa = reinterpret_cast<const uint4*>(w.packed) + ra * blocks * 4 + t;
-    const uint4* pb = reinterpret_cast<const uint4*>(w.packed) + rb * blocks * 4 + t;
-    const T* scales = static_cast<const T*>(w.scales);
-    float sum[NT][4] = {};
-    for (uint64_t b = warp; b < blocks; b += kWarps) {
-        const uint4 qa = pa[b * 4], qb = pb[b * 4];
-        const uint32_t wa[4] = {qa.x, qa.y, qa.z, qa.w}, wb[4] = {qb.x, qb.y, qb.z, qb.w};
-#pragma unroll
-        for (int sub = 0; sub < SUB; sub++) {
-            const uint64_t group = (b * 128 + sub * (128 / SUB)) >> w.group_log2;
-            if (group >= groups) break;
-            const float sa = Half<T>::to_float(scales[group * w.n + ra]), sb = Half<T>::to_float(scales[group * w.n + rb]);
-            const uint32_t za = Half<T>::kOne + 0x10001u * (w.zeros ? w.zeros[group * w.n + ra] : 8u);
-            const uint32_t zb = Half<T>::kOne + 0x10001u * (w.zeros ? w.zeros[group * w.n + rb] : 8u);
-            float part[NT][4] = {};
-#pragma unroll
-            for (int j = sub * 4 / SUB; j < (sub + 1) * 4 / SUB; j++) {
-                uint32_t a[4], c[4];
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    a[i] = Half<T>::sub2(((wa[j] >> (4 * i)) & 0x000f000fu) | Half<T>::kOne, za);
-                    c[i] = Half<T>::sub2(((wb[j] >> (4 * i)) & 0x000f000fu) | Half<T>::kOne, zb);
-                }
-#pragma unroll
-                for (int i = 0; i < NT; i++) {
-                    const uint64_t tok = m0 + i * 8 + g;
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (tok < m) v = load_x(x + tok * ldx, b * 128 + j * 32 + t * 8, kx);
-                    Half<T>::mma(part[i], a[0], c[0], a[1], c[1], v.x, v.y);
-                    Half<T>::mma(part[i], a[2], c[2], a[3], c[3], v.z, v.w);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < NT; i++) {
-                sum[i][0] = fmaf(sa, part[i][0], sum[i][0]);
-                sum[i][1] = fmaf(sa, part[i][1], sum[i][1]);
-                sum[i][2] = fmaf(sb, part[i][2], sum[i][2]);
-                sum[i][3] = fmaf(sb, part[i][3], sum[i][3]);
-            }
-        }
+__device__ __forceinline__ void mma_bytes(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Shape of a block: W warps that each work on R rows of tiles, with NT * 8
+// columns of the matrix instruction and D slots of BT tile columns in flight.
+// DIGITS: the activations as whole numbers, three columns each; see below.
+template <bool DIGITS_, int NT_, int W_, int R_, int BT_, int D_>
+struct Shape {
+    static constexpr bool DIGITS = DIGITS_;
+    static constexpr int NT = NT_, W = W_, R = R_, BT = BT_, D = D_;
+    static constexpr int kTokens = DIGITS ? 8 * NT / 3 : 8 * NT;        // rows of activations at a time
+    static constexpr int kColumns = DIGITS ? 3 : 1;                     // matrix columns of one of them
+    static constexpr int kRowBytes = DIGITS ? 128 : 256;                // of a column, per tile
+    static constexpr int kSlot = BT * R * 1024;                         // bytes
+    static constexpr int kRing = W * D * kSlot, kBars = W * D * 8 + 16;
+    static constexpr int kBuffers = DIGITS ? 1 : 2;                     // chunks of activations held
+    static_assert(16 * R * 8 * NT * 4 <= D * kSlot, "a warp's sums have to fit in its slots");
+    // Shared memory a tile column of activations takes, and what does not
+    // depend on their number.
+    static constexpr uint64_t per_tile(uint64_t tokens, int sub) {
+        return kBuffers * tokens * kColumns * kRowBytes + (DIGITS ? sub * NT * 64 : 0);
     }
-#pragma unroll
-    for (int i = 0; i < NT; i++) {
-        s_sum[warp][g][i * 8 + 2 * t] = sum[i][0];
-        s_sum[warp][g][i * 8 + 2 * t + 1] = sum[i][1];
-        s_sum[warp][g + 8][i * 8 + 2 * t] = sum[i][2];
-        s_sum[warp][g + 8][i * 8 + 2 * t + 1] = sum[i][3];
+    static constexpr uint64_t fixed(uint64_t tokens) { return kRing + kBars + kBuffers * tokens * kColumns * 64; }
+};
+
+// y = values * x for the rows of tiles of this block.
+//
+// The weights stream through shared memory: lane 0 of each warp keeps D slots
+// filled with asynchronous bulk copies (contiguous, thanks to the layout), so
+// 64 to 128 KiB per SM are in flight and none of it takes registers.  The
+// activations of a chunk of columns lie in shared memory.  When a block has
+// fewer rows than warps, teams of warps share a row, each with a run of every
+// chunk's columns, and their sums are added in a fixed order.
+//
+// Few rows are bound by the instructions that unpack the codes, and there are
+// two ways to feed the matrix instruction:
+//
+// * In 16 bits: the differences code - zero, exact, times x, exact products
+//   summed in float; the scale of a group (128 / SUB columns, or a multiple of
+//   128 with SUB = 1) multiplies the group's sum.  Eleven instructions per
+//   eight codes.
+// * DIGITS, for one or two rows of activations: codes as bytes, three
+//   instructions per eight.  x of a group is written as whole numbers of
+//   2^(e-21), e the exponent of its largest magnitude, and those as three
+//   signed bytes (hi * 2^16 + mid * 2^8 + lo), a column of the matrix
+//   instruction each.  A bfloat16 down to 2^-14 of the group's largest is
+//   exact, anything smaller off by 2^-22 of the largest at most.  Sums are
+//   whole numbers, exact in 32 bits, and so is the zero's part, zero * sum of
+//   digits.
+template <class T, class S, int SUB, bool ZEROS>
+__global__ void __launch_bounds__(S::W * 32, 1)
+qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias, void* y, uint64_t ldy, int y_float,
+                int x_vec, uint32_t chunk_tiles) {
+    constexpr bool DIGITS = S::DIGITS;
+    constexpr int NT = S::NT, W = S::W, R = S::R, BT = S::BT, D = S::D, kPer = (SUB + 1) / 2;
+    using Sum = std::conditional_t<DIGITS, int, float>;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ int s_failed;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const uint64_t m0 = (uint64_t)blockIdx.y * S::kTokens;
+    const int tokens = (int)min((uint64_t)S::kTokens, m - m0), columns = tokens * S::kColumns;
+    const uint32_t tiles = (uint32_t)((w.k + 127) / 128);
+    const uint32_t groups = (uint32_t)((w.k + (1ull << w.group_log2) - 1) >> w.group_log2);
+    const uint32_t chunks = (tiles + chunk_tiles - 1) / chunk_tiles;
+    const uint64_t row_tiles = (w.n + 15) / 16, units = (row_tiles + R - 1) / R;
+    const uint32_t pitch = chunk_tiles * S::kRowBytes + 64;     // columns of activations, apart in the banks
+    unsigned char* const ring = smem + warp * (D * S::kSlot);
+    const uint32_t smem_at = (uint32_t)__cvta_generic_to_shared(smem);
+    const uint32_t ring_at = smem_at + warp * (D * S::kSlot), bars = smem_at + S::kRing + warp * (D * 8);
+    const uint32_t x_bars = smem_at + S::kRing + W * D * 8;     // two: a chunk of activations is there
+    unsigned char* const xs = smem + S::kRing + S::kBars;
+    // DIGITS: per tile, group and pair of columns, the digits' sums and the unit of x
+    int4* const info = reinterpret_cast<int4*>(xs + columns * pitch);
+
+    if (threadIdx.x == 0) {
+        s_failed = 0;
+        qrc::mbar_init(x_bars, 1);
+        qrc::mbar_init(x_bars + 8, 1);
+    }
+    if (lane == 0) {
+        for (int i = 0; i < D; i++) qrc::mbar_init(bars + 8 * i, 1);
+        qrc::fence_mbar_init();
+        qrc::fence_proxy_async_smem();
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * 8 * NT; i += kWarps * 32) {
-        const int r = i & 15, c = i >> 4;
-        const uint64_t row = n0 + r, tok = m0 + c;
-        if (row >= w.n || tok >= m) continue;
-        float v = 0.0f;
+    qrc::griddep_wait();
+    qrc::griddep_launch_dependents();
+
+    // Eight activations from column k0 on, zero behind the last column.
+    auto load_x = [&](int tok, uint64_t k0) {
+        const T* p = x + (m0 + tok) * ldx + k0;
+        if (x_vec && k0 + 8 <= w.k) return *reinterpret_cast<const uint4*>(p);
+        uint32_t e[8];
 #pragma unroll
-        for (int j = 0; j < kWarps; j++) v += s_sum[j][r][c];
-        if (bias) v += Half<T>::to_float(bias[row]);
-        if (y_float) static_cast<float*>(y)[tok * ldy + row] = v;
-        else static_cast<T*>(y)[tok * ldy + row] = Half<T>::round(v);
+        for (int j = 0; j < 8; j++) e[j] = k0 + j < w.k ? reinterpret_cast<const uint16_t*>(p)[j] : 0u;
+        return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+    };
+    // Brings a chunk's activations to shared memory, zero behind column k.
+    auto stage_half = [&](uint32_t chunk, int buffer) {
+        const uint32_t tile0 = chunk * chunk_tiles, n16 = min(chunk_tiles, tiles - tile0) * 16;
+        unsigned char* const to = xs + buffer * (columns * pitch);
+        const uint64_t k0 = (uint64_t)tile0 * 128;
+        // Aligned rows: one bulk copy each; the last eight columns, if not whole, by hand.
+        const uint32_t whole = x_vec ? (uint32_t)(min((uint64_t)n16 * 8, w.k - k0) / 8) : 0;
+        if (threadIdx.x == 0) {
+            qrc::fence_proxy_async_smem();                      // the buffer has been read: before its refill
+            qrc::mbar_arrive_expect_tx(x_bars + 8 * buffer, whole * 16 * tokens);
+            if (whole)
+                for (int tok = 0; tok < tokens; tok++)
+                    qrc::bulk_g2s(smem_at + (uint32_t)(to - smem) + tok * pitch, (uint64_t)(x + (m0 + tok) * ldx + k0),
+                                  whole * 16, x_bars + 8 * buffer);
+        }
+        const uint32_t rest = n16 - whole;
+#pragma unroll 4
+        for (uint32_t i = threadIdx.x; i < rest * tokens; i += W * 32) {
+            const uint32_t tok = i / rest, c = whole + i - tok * rest;
+            *reinterpret_cast<uint4*>(to + tok * pitch + c * 16) = load_x(tok, k0 + c * 8);
+        }
+    };
+    // The same as three bytes per activation, with the sums of the bytes.
+    auto stage_digits = [&](uint32_t chunk) {
+        const uint32_t tile0 = chunk * chunk_tiles, n16 = min(chunk_tiles, tiles - tile0) * 16, padded = (n16 + 31) / 32 * 32;
+        constexpr int kLanes = 16 / SUB;                        // lanes of a group, eight columns each
+        // Whole warps take part, and a group lies within one: rows are padded to 32 lanes.
+        for (uint32_t i = threadIdx.x; i < padded * tokens; i += W * 32) {
+            const uint32_t tok = i / padded, c = i - tok * padded;
+            const uint64_t k0 = (uint64_t)tile0 * 128 + c * 8;
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (c < n16 && k0 < w.k) v = load_x(tok, k0);
+            float f[8];
+            const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+            uint32_t most = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                f[j] = Half<T>::to_float(from_bits<T>(j & 1 ? word[j / 2] >> 16 : word[j / 2] & 0xffffu));
+                most = max(most, __float_as_uint(f[j]) & 0x7fffffffu);
+            }
+#pragma unroll
+            for (int d = kLanes / 2; d; d >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, d));
+            // 2^(21 - e), e at least -105: smaller activations keep fewer bits
+            const uint32_t e = max(most >> 23, 22u);
+            const float to_whole = __uint_as_float((275u - e) << 23);
+            const bool bad = most >= 0x7f800000u;               // an infinity or NaN: the group counts as NaN
+            uint32_t q[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++)                         // rounded by the addition, digits biased by 128
+                q[j] = bad ? 0x808080u : __float_as_uint(fmaf(f[j], to_whole, 12582912.0f)) + (0x808080u - 0x4b400000u);
+            int4 sums = make_int4(0, 0, 0, 0);
+            unsigned char* const to = xs + tok * 3 * pitch + (c >> 4) * 128 + ((c >> 3) & 1) * 64 + (c & 3) * 16 + ((c >> 2) & 1) * 8;
+#pragma unroll
+            for (int p = 0; p < 3; p++) {                       // hi, mid, lo
+                const uint32_t pick = (2 - p) | (6 - p) << 4;
+                const uint32_t b04 = __byte_perm(q[0], q[4], pick), b15 = __byte_perm(q[1], q[5], pick);
+                const uint32_t b26 = __byte_perm(q[2], q[6], pick), b37 = __byte_perm(q[3], q[7], pick);
+                const uint32_t first = __byte_perm(b04, b15, 0x5410) ^ 0x80808080u, second = __byte_perm(b26, b37, 0x5410) ^ 0x80808080u;
+                if (c < n16) *reinterpret_cast<uint2*>(to + p * pitch) = make_uint2(first, second);
+                int d = __dp4a((int)first, 0x01010101, __dp4a((int)second, 0x01010101, 0));
+#pragma unroll
+                for (int step = kLanes / 2; step; step >>= 1) d += __shfl_xor_sync(0xffffffffu, d, step);
+                (p == 0 ? sums.x : p == 1 ? sums.y : sums.z) = d;
+            }
+            if (c < n16 && c % kLanes == 0) {
+                // unit 2^(e - 21), over the 8 that the codes are multiplied by
+                const float unit = bad ? __int_as_float(0x7fffffff) : __uint_as_float(e << 23) * 0x1p-24f;
+                const int digit[3] = {sums.x, sums.y, sums.z};
+#pragma unroll
+                for (int p = 0; p < 3; p++) {
+                    const uint32_t col = tok * 3 + p;
+                    int* const at = reinterpret_cast<int*>(info + (c / kLanes * NT + (col >> 3)) * 4 + ((col & 7) >> 1));
+                    at[col & 1] = digit[p];
+                    at[2 + (col & 1)] = __float_as_int(unit);
+                }
+            }
+        }
+    };
+
+    // Lanes without a column repeat the last one; what they sum is not stored.
+    uint32_t x_at[NT];
+#pragma unroll
+    for (int i = 0; i < NT; i++) x_at[i] = min(i * 8 + g, columns - 1) * pitch;
+    const uint64_t u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
+    const uint32_t rows = (uint32_t)(u1 - u0), passes = (rows + W - 1) / W, per_pass = (rows + passes - 1) / passes;
+    uint32_t parity = 0, x_parity = 0;
+    bool failed = false, staged = false;
+    for (uint32_t pass = 0; pass < passes; pass++) {
+        const uint32_t first = pass * per_pass, here = min(per_pass, rows - first);
+        const uint32_t team = W / here, mine = warp / team, member = warp - mine * team;
+        const bool active = mine < here;
+        const uint64_t unit = u0 + first + (active ? mine : 0);
+        const uint4* src[R];
+        const uint16_t* scale_at[R];
+        const uint8_t* zero_at[R];
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            // Rows behind the last one repeat it; their sums are not stored.
+            const uint64_t rt = min(unit * R + r, row_tiles - 1), row = min(rt * 16 + (lane & 15), w.n - 1);
+            src[r] = reinterpret_cast<const uint4*>(w.packed) + rt * tiles * 64;
+            scale_at[r] = static_cast<const uint16_t*>(w.scales) + row;
+            zero_at[r] = w.zeros + row;
+        }
+        // This warp's tile columns of a chunk: a run of them.
+        auto run_of = [&](uint32_t chunk, uint32_t& lo, uint32_t& hi) {
+            const uint32_t size = min(chunk_tiles, tiles - chunk * chunk_tiles);
+            lo = active ? size * member / team : 0;
+            hi = active ? size * (member + 1) / team : 0;
+        };
+        // The copies run ahead of the product, across the chunks.
+        uint32_t ahead_chunk = 0, ahead_at = 0, ahead_left = 0, filled = 0;
+        auto settle = [&]() {
+            while (ahead_left == 0 && ahead_chunk < chunks) {
+                uint32_t lo, hi;
+                run_of(ahead_chunk, lo, hi);
+                ahead_at = ahead_chunk * chunk_tiles + lo;
+                ahead_left = hi - lo;
+                ahead_chunk++;
+            }
+        };
+        auto fetch = [&](int slot) {
+            const uint32_t n = min((uint32_t)BT, ahead_left);
+            if (lane == 0) {
+                qrc::fence_proxy_async_smem();                  // the slot has been read: before its refill
+                qrc::mbar_arrive_expect_tx(bars + 8 * slot, n * R * 1024);
+#pragma unroll
+                for (int r = 0; r < R; r++)
+                    qrc::bulk_g2s(ring_at + slot * S::kSlot + r * BT * 1024, (uint64_t)(src[r] + (uint64_t)ahead_at * 64),
+                                  n * 1024, bars + 8 * slot);
+            }
+            filled |= 1u << slot;
+            ahead_at += n;
+            ahead_left -= n;
+            if (!ahead_left) settle();
+        };
+        // Scales and zeros of a batch, one row and group per lane: those of
+        // row lane % 16 and group 2 * i + lane / 16 of a tile.
+        uint32_t scale[BT][R][kPer], zero[BT][R][kPer];
+        auto load_scales = [&](uint32_t tile) {
+#pragma unroll
+            for (int b = 0; b < BT; b++) {
+#pragma unroll
+                for (int i = 0; i < kPer; i++) {
+                    const uint32_t sub = SUB == 1 ? 0 : 2 * i + (lane >> 4);
+                    // Groups behind the last one repeat it: their sums are 0.
+                    const uint32_t group = min(SUB == 1 ? (tile + b) >> (w.group_log2 - 7) : (tile + b) * SUB + sub, groups - 1);
+#pragma unroll
+                    for (int r = 0; r < R; r++) {
+                        scale[b][r][i] = __ldg(scale_at[r] + (uint64_t)group * (uint32_t)w.n);
+                        if (ZEROS) zero[b][r][i] = __ldg(zero_at[r] + (uint64_t)group * (uint32_t)w.n);
+                    }
+                }
+            }
+        };
+
+        float sum[R][NT][4] = {};
+        settle();
+        for (int i = 0; i < D && ahead_left && !failed; i++) fetch(i);
+        int slot = 0;
+        if (!DIGITS && chunks && (!staged || chunks > 1)) {
+            if (pass) __syncthreads();                          // everyone is done with the last pass
+            stage_half(0, 0);
+        }
+        for (uint32_t chunk = 0; chunk < chunks; chunk++) {
+            uint32_t lo, hi;
+            run_of(chunk, lo, hi);
+            if (lo < hi) load_scales(chunk * chunk_tiles + lo);
+            const int buffer = DIGITS ? 0 : chunk & 1;
+            if (!staged || chunks > 1) {
+                if (DIGITS) {
+                    if (pass || chunk) __syncthreads();         // everyone is done with the last chunk
+                    stage_digits(chunk);
+                }
+                // What was staged by hand is there for all, and everyone is
+                // done with the chunk before this one, whose buffer is next.
+                __syncthreads();
+                if (!DIGITS) {
+                    if (chunk + 1 < chunks) stage_half(chunk + 1, buffer ^ 1);
+                    if (!qrc::mbar_wait_bounded(x_bars + 8 * buffer, (x_parity >> buffer) & 1)) failed = true;
+                    x_parity ^= 1u << buffer;
+                }
+                staged = true;
+            }
+            const unsigned char* xt = xs + buffer * (columns * pitch) + lo * S::kRowBytes + t * 16;
+            const int4* it = info + lo * (SUB * NT * 4) + t;
+            for (uint32_t at = lo; at < hi; at += BT, xt += BT * S::kRowBytes, it += BT * SUB * NT * 4) {
+                uint32_t scale_now[BT][R][kPer], zero_now[BT][R][kPer];
+#pragma unroll
+                for (int b = 0; b < BT; b++) {
+#pragma unroll
+                    for (int r = 0; r < R; r++) {
+#pragma unroll
+                        for (int i = 0; i < kPer; i++) {
+                            scale_now[b][r][i] = scale[b][r][i];
+                            if (ZEROS) zero_now[b][r][i] = zero[b][r][i];
+                        }
+                    }
+                }
+                if (at + BT < hi) load_scales(chunk * chunk_tiles + at + BT);
+                if (failed || !qrc::mbar_wait_bounded(bars + 8 * slot, (parity >> slot) & 1)) { failed = true; break; }
+                parity ^= 1u << slot;
+                filled &= ~(1u << slot);
+                const unsigned char* q = ring + slot * S::kSlot + lane * 16;
+                // Tile columns behind the run hold nothing of use: they are left out.
+#pragma unroll
+                for (int b = 0; b < BT; b++) {
+                    if (at + b >= hi) break;
+                    uint32_t top[R][4], low[R][4];
+#pragma unroll
+                    for (int r = 0; r < R; r++) {
+                        *reinterpret_cast<uint4*>(top[r]) = *reinterpret_cast<const uint4*>(q + (r * BT + b) * 1024);
+                        *reinterpret_cast<uint4*>(low[r]) = *reinterpret_cast<const uint4*>(q + (r * BT + b) * 1024 + 512);
+                    }
+                    uint4 v[NT];
+#pragma unroll
+                    for (int sub = 0; sub < SUB; sub++) {
+                        const int from = SUB == 1 ? 0 : (sub & 1) * 16;
+                        float sa[R], sb[R];
+                        uint32_t za[R], zb[R];
+#pragma unroll
+                        for (int r = 0; r < R; r++) {
+                            sa[r] = Half<T>::to_float(from_bits<T>(__shfl_sync(0xffffffffu, scale_now[b][r][sub / 2], from + g)));
+                            sb[r] = Half<T>::to_float(from_bits<T>(__shfl_sync(0xffffffffu, scale_now[b][r][sub / 2], from + g + 8)));
+                            za[r] = ZEROS ? __shfl_sync(0xffffffffu, zero_now[b][r][sub / 2], from + g) * 8 : 64u;
+                            zb[r] = ZEROS ? __shfl_sync(0xffffffffu, zero_now[b][r][sub / 2], from + g + 8) * 8 : 64u;
+                            if (!DIGITS) {
+                                za[r] = za[r] * 0x10001u | Half<T>::kOne;
+                                zb[r] = zb[r] * 0x10001u | Half<T>::kOne;
+                            }
+                        }
+                        Sum part[R][NT][4] = {};
+#pragma unroll
+                        for (int j = sub * 4 / SUB; j < (sub + 1) * 4 / SUB; j++) {
+#pragma unroll
+                            for (int i = 0; i < NT; i++) {
+                                if (!DIGITS) v[i] = *reinterpret_cast<const uint4*>(xt + x_at[i] + b * 256 + j * 64);
+                                else if (j % 2 == 0) v[i] = *reinterpret_cast<const uint4*>(xt + x_at[i] + b * 128 + j * 32);
+                            }
+#pragma unroll
+                            for (int r = 0; r < R; r++) {
+                                const uint32_t wt = top[r][j], wl = low[r][j];
+                                if constexpr (DIGITS) {
+                                    const uint32_t a[4] = {wt & 0x78787878u, wl & 0x78787878u,
+                                                           rotate_right(wt, 4) & 0x78787878u, rotate_right(wl, 4) & 0x78787878u};
+#pragma unroll
+                                    for (int i = 0; i < NT; i++) mma_bytes(part[r][i], a, j % 2 ? v[i].z : v[i].x, j % 2 ? v[i].w : v[i].y);
+                                } else {
+                                    uint32_t a[2][4];
+#pragma unroll
+                                    for (int h = 0; h < 2; h++) {
+                                        a[h][0] = Half<T>::sub2(code_pair<T>(wt, 2 * h), za[r]);
+                                        a[h][1] = Half<T>::sub2(code_pair<T>(wl, 2 * h), zb[r]);
+                                        a[h][2] = Half<T>::sub2(code_pair<T>(wt, 2 * h + 1), za[r]);
+                                        a[h][3] = Half<T>::sub2(code_pair<T>(wl, 2 * h + 1), zb[r]);
+                                    }
+#pragma unroll
+                                    for (int i = 0; i < NT; i++) {
+                                        Half<T>::mma(part[r][i], a[0], v[i].x, v[i].y);
+                                        Half<T>::mma(part[r][i], a[1], v[i].z, v[i].w);
+                                    }
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < NT; i++) {
+                            int4 of = make_int4(0, 0, 0, 0);
+                            if (DIGITS) of = it[((b * SUB + sub) * NT + i) * 4];
+#pragma unroll
+                            for (int r = 0; r < R; r++) {
+                                if constexpr (DIGITS) {
+                                    const float f0 = __int_as_float(of.z), f1 = __int_as_float(of.w);
+                                    sum[r][i][0] = fmaf(sa[r] * f0, (float)(part[r][i][0] - (int)za[r] * of.x), sum[r][i][0]);
+                                    sum[r][i][1] = fmaf(sa[r] * f1, (float)(part[r][i][1] - (int)za[r] * of.y), sum[r][i][1]);
+                                    sum[r][i][2] = fmaf(sb[r] * f0, (float)(part[r][i][2] - (int)zb[r] * of.x), sum[r][i][2]);
+                                    sum[r][i][3] = fmaf(sb[r] * f1, (float)(part[r][i][3] - (int)zb[r] * of.y), sum[r][i][3]);
+                                } else {
+                                    add_scaled<NT>(sum[r][i][0], sum[r][i][1], sa[r], part[r][i][0], part[r][i][1]);
+                                    add_scaled<NT>(sum[r][i][2], sum[r][i][3], sb[r], part[r][i][2], part[r][i][3]);
+                                }
+                            }
+                        }
+                    }
+                }
+                __syncwarp();
+                if (ahead_left) fetch(slot);
+                slot = slot + 1 == D ? 0 : slot + 1;
+            }
+        }
+        if (failed) {                                           // a wait gave up: wait, bounded, for what is under way
+            s_failed = 1;
+            for (int i = 0; i < D; i++)
+                if (filled >> i & 1) qrc::mbar_wait_bounded(bars + 8 * i, (parity >> i) & 1);
+            filled = 0;
+            for (int i = 0; i < 2; i++) qrc::mbar_wait_bounded(x_bars + 8 * i, (x_parity >> i & 1) ^ 1);
+        }
+
+        // The sums of a team meet in its slots, which hold nothing any more.
+        float* const out = reinterpret_cast<float*>(ring);      // [8 * NT][16 * R]
+        if (active) {
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+#pragma unroll
+                for (int i = 0; i < NT; i++) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) out[(i * 8 + 2 * t + (e & 1)) * (16 * R) + r * 16 + g + (e >> 1) * 8] = sum[r][i][e];
+                }
+            }
+        }
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < here * tokens * 16 * R; i += W * 32) {
+            const uint32_t r = i % (16 * R), tok = i / (16 * R) % tokens, which = i / (16 * R * tokens);
+            const uint64_t row = (u0 + first + which) * 16 * R + r;
+            if (row >= w.n) continue;
+            float v[S::kColumns] = {};
+            for (uint32_t j = 0; j < team; j++) {
+                const float* part = reinterpret_cast<const float*>(smem + (which * team + j) * (D * S::kSlot)) +
+                                    tok * S::kColumns * (16 * R) + r;
+#pragma unroll
+                for (int p = 0; p < S::kColumns; p++) v[p] += part[p * (16 * R)];
+            }
+            float all = v[0] * (DIGITS ? 65536.0f : 1.0f / Half<T>::kUnit);
+            if constexpr (DIGITS) all += v[1] * 256.0f + v[2];
+            if (bias) all += Half<T>::to_float(bias[row]);
+            if (s_failed) all = __int_as_float(0x7fffffff);     // NaN: no valid result
+            if (y_float) static_cast<float*>(y)[(m0 + tok) * ldy + row] = all;
+            else static_cast<T*>(y)[(m0 + tok) * ldy + row] = Half<T>::round(all);
+        }
+        if (pass + 1 < passes) __syncthreads();                 // before the slots are filled again
     }
 }
 
@@ -325,7 +697,7 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t kx, uint64_t m, c
 // Host side
 // ---------------------------------------------------------------------------
 
-constexpr uint64_t kMaxSide = 1ull << 31;     // rows or columns of a matrix, rows of activations
+constexpr uint64_t kMaxSide = 0x7fffffffu;    // rows or columns of a matrix, rows of activations
 
 bool valid_w4(const qrc_w4* w) {
     if (!w || (w->type != QRC_BF16 && w->type != QRC_F16)) return false;
@@ -362,57 +734,56 @@ dim3 grid_for(uint64_t items, uint64_t per_block) {
     return dim3((unsigned)std::min<uint64_t>((items + per_block - 1) / per_block, 1u << 16));
 }
 
-template <class T>
-cudaError_t launch_matvec(const qrc_w4& w, const T* x, uint64_t ldx, uint64_t kx, uint64_t m, const T* bias, void* y,
-                          uint64_t ldy, int y_float, cudaStream_t s) {
+// Shared memory a block may have, and what its static part takes.
+constexpr int kSmemLimit = 227 * 1024 - 64;
+
+template <class T, class S>
+int launch_shape(const qrc_w4& w, const T* x, uint64_t ldx, uint64_t m, const T* bias, void* y, uint64_t ldy,
+                 int y_float, int sms, cudaStream_t s) {
     const W4 a = {w.d_packed, w.d_scales, w.d_zeros, w.n, w.k, log2_of(w.group)};
-    const int nt = m <= 8 ? 1 : m <= 16 ? 2 : 4;
-    auto go = [&](auto kernel) {
-        // grid.y has room for 65,535 slices of activations per launch
-        for (uint64_t m0 = 0; m0 < m; m0 += 65535ull * 8 * nt) {
-            const uint64_t rows = std::min<uint64_t>(m - m0, 65535ull * 8 * nt);
-            void* to = static_cast<char*>(y) + m0 * ldy * (y_float ? 4 : 2);
-            const cudaError_t e = launch_overlapped(
-                kernel, dim3((unsigned)((w.n + 15) / 16), (unsigned)((rows + 8 * nt - 1) / (8 * nt))), kWarps * 32, 0, s,
-                1, a, x + m0 * ldx, ldx, kx, rows, bias, to, ldy, y_float);
-            if (e != cudaSuccess) return e;
-        }
-        return cudaSuccess;
+    const int x_vec = rows_aligned(x, ldx, m, 2), sub = w.group == 32 ? 4 : w.group == 64 ? 2 : 1;
+    const uint64_t tiles = (w.k + 127) / 128, units = ((w.n + 15) / 16 + S::R - 1) / S::R;
+    const uint64_t tokens = std::min<uint64_t>(m, S::kTokens);
+    // As many columns at a time as fit beside the ring, in chunks of one size.
+    const uint64_t most = (kSmemLimit - S::fixed(tokens)) / S::per_tile(tokens, sub);
+    const uint64_t chunks = std::max<uint64_t>((tiles + most - 1) / most, 1);
+    const uint32_t chunk_tiles = (uint32_t)std::max<uint64_t>((tiles + chunks - 1) / chunks, 1);
+    const size_t smem = S::fixed(tokens) + chunk_tiles * S::per_tile(tokens, sub);
+    const dim3 grid((unsigned)std::min<uint64_t>(units, sms), (unsigned)((m + S::kTokens - 1) / S::kTokens));
+    auto go = [&](auto kernel) -> int {
+        QRC_CK(grant_smem((const void*)kernel, kSmemLimit));
+        QRC_CK(launch_overlapped(kernel, grid, S::W * 32, smem, s, 1, a, x, ldx, m, bias, y, ldy, y_float, x_vec, chunk_tiles));
+        return QRC_OK;
     };
-    auto by_sub = [&](auto n) {
-        constexpr int NT = decltype(n)::value;
-        switch (w.group) {
-            case 32: return go(qrc_k_w4_matvec<T, NT, 4>);
-            case 64: return go(qrc_k_w4_matvec<T, NT, 2>);
-            default: return go(qrc_k_w4_matvec<T, NT, 1>);
-        }
-    };
-    switch (nt) {
-        case 1: return by_sub(std::integral_constant<int, 1>());
-        case 2: return by_sub(std::integral_constant<int, 2>());
-        default: return by_sub(std::integral_constant<int, 4>());
+    switch (sub) {
+        case 4: return w.d_zeros ? go(qrc_k_w4_matvec<T, S, 4, true>) : go(qrc_k_w4_matvec<T, S, 4, false>);
+        case 2: return w.d_zeros ? go(qrc_k_w4_matvec<T, S, 2, true>) : go(qrc_k_w4_matvec<T, S, 2, false>);
+        default: return w.d_zeros ? go(qrc_k_w4_matvec<T, S, 1, true>) : go(qrc_k_w4_matvec<T, S, 1, false>);
     }
 }
 
 template <class T>
-cudaError_t lay_out_and_multiply(const qrc_w4& w, const void* d_x, uint64_t m, uint64_t ldx, const void* d_bias,
-                                 void* d_y, uint64_t ldy, int y_float, void* d_work, cudaStream_t s) {
-    const T* x = static_cast<const T*>(d_x);
-    uint64_t kx = w.k;
-    if (d_work) {
-        const uint64_t width = (w.k + 127) / 128 * 128;
-        const cudaError_t e = launch_overlapped(qrc_k_w4_lay_out<T>, grid_for(m * width, 256), 256, 0, s, 1, x, ldx, m,
-                                                w.k, static_cast<T*>(d_work));
-        if (e != cudaSuccess) return e;
-        x = static_cast<const T*>(d_work);
-        ldx = kx = width;
+int launch_matvec(const qrc_w4& w, const void* d_x, uint64_t m, uint64_t ldx, const void* d_bias, void* d_y,
+                  uint64_t ldy, int y_float, int sms, cudaStream_t s) {
+    const T* bias = static_cast<const T*>(d_bias);
+    // grid.y has room for 65,535 slices of activations per launch
+    const uint64_t step = 65535ull * 32;
+    for (uint64_t m0 = 0; m0 < m; m0 += step) {
+        const uint64_t rows = std::min(m - m0, step);
+        const T* x = static_cast<const T*>(d_x) + m0 * ldx;
+        void* y = static_cast<char*>(d_y) + m0 * ldy * (y_float ? 4 : 2);
+        auto go = [&](auto shape) { return launch_shape<T, decltype(shape)>(w, x, ldx, rows, bias, y, ldy, y_float, sms, s); };
+        const int rc = rows <= 2 ? go(Shape<true, 1, 16, 1, 4, 2>())
+                       : rows <= 8 ? go(Shape<false, 1, 16, 1, 4, 2>())
+                       : rows <= 16 ? go(Shape<false, 2, 16, 1, 4, 2>()) : go(Shape<false, 4, 8, 2, 2, 2>());
+        if (rc != QRC_OK) return rc;
     }
-    return launch_matvec<T>(w, x, ldx, kx, m, static_cast<const T*>(d_bias), d_y, ldy, y_float, s);
+    return QRC_OK;
 }
 
 template <class T>
 cudaError_t launch_dequant(const qrc_w4& w, void* out, uint64_t ld, int type, cudaStream_t s) {
-    const uint64_t words = w.n * ((w.k + 127) / 128 * 16);
+    const uint64_t words = qrc_w4_words(w.n, w.k);
     const int vec = rows_aligned(out, ld, w.n, type == QRC_F32 ? 4 : 2);
     const T* scales = static_cast<const T*>(w.d_scales);
     auto go = [&](auto* to) {
@@ -431,14 +802,14 @@ cudaError_t launch_dequant(const qrc_w4& w, void* out, uint64_t ld, int type, cu
 template <class T>
 cudaError_t launch_quant(const qrc_w4& w, const void* d_w, uint64_t ld, int symmetric, cudaStream_t s) {
     const int vec = rows_aligned(d_w, ld, w.n, 2);
-    return launch_overlapped(qrc_k_w4_quant<T>, grid_for(w.n * ((w.k + 255) / 256), 8), 256, 0, s, 1,
+    return launch_overlapped(qrc_k_w4_quant<T>, grid_for((w.n + 15) / 16 * 16 * ((w.k + 255) / 256), 8), 256, 0, s, 1,
                              static_cast<const T*>(d_w), ld, w.n, w.k, w.group, symmetric, vec, w.d_packed,
                              static_cast<T*>(w.d_scales), w.d_zeros);
 }
 
 }  // namespace
 
-QRC_API uint64_t qrc_w4_words(uint64_t n, uint64_t k) { return n * ((k + 127) / 128 * 16); }
+QRC_API uint64_t qrc_w4_words(uint64_t n, uint64_t k) { return (n + 15) / 16 * ((k + 127) / 128) * 256; }
 
 QRC_API int qrc_w4_quant(int device, const void* d_w, uint64_t ld, int symmetric, const qrc_w4* w, void* stream) {
     if (!valid_w4(w) || (w->n > 1 && ld < w->k)) return QRC_ERR_INVALID;
@@ -481,13 +852,8 @@ QRC_API int qrc_w4_dequant(int device, const qrc_w4* w, void* d_out, uint64_t ld
     return QRC_OK;
 }
 
-QRC_API size_t qrc_w4_matvec_workspace(const qrc_w4* w, const void* d_x, uint64_t m, uint64_t ldx) {
-    if (!valid_w4(w) || m > kMaxSide || !m || !w->n || !w->k || rows_aligned(d_x, ldx, m, 2)) return 0;
-    return m * ((w->k + 127) / 128 * 128) * 2;
-}
-
 QRC_API int qrc_w4_matvec(int device, const qrc_w4* w, const void* d_x, uint64_t m, uint64_t ldx, const void* d_bias,
-                          void* d_y, uint64_t ldy, int y_type, void* d_work, void* stream) {
+                          void* d_y, uint64_t ldy, int y_type, void* stream) {
     if (!valid_w4(w) || m > kMaxSide || (m > 1 && (ldx < w->k || ldy < w->n))) return QRC_ERR_INVALID;
     if (y_type != QRC_F32 && y_type != w->type) return QRC_ERR_INVALID;
     if (((uintptr_t)d_x & 1) || ((uintptr_t)d_bias & 1) || ((uintptr_t)d_y & (y_type == QRC_F32 ? 3 : 1)))
@@ -496,17 +862,13 @@ QRC_API int qrc_w4_matvec(int device, const qrc_w4* w, const void* d_x, uint64_t
     const uint64_t y_bytes = span(m, w->n, ldy, y_type == QRC_F32 ? 4 : 2);
     if (touches(*w, d_y, y_bytes) || overlap(d_y, y_bytes, d_x, span(m, w->k, ldx, 2)) ||
         overlap(d_y, y_bytes, d_bias, w->n * 2)) return QRC_ERR_INVALID;
-    const size_t need = qrc_w4_matvec_workspace(w, d_x, m, ldx);
-    if (need && (!d_work || ((uintptr_t)d_work & 15))) return QRC_ERR_INVALID;
-    if (!sm100_sms(device)) return QRC_ERR_DEVICE;
+    const int sms = sm100_sms(device);
+    if (!sms) return QRC_ERR_DEVICE;
     if (!m || !w->n) return QRC_OK;
     DeviceScope scope(device);
     if (!scope.ok) return QRC_ERR_DEVICE;
     cudaStream_t s = as_stream(stream);
-    void* work = need ? d_work : nullptr;
     const int y_float = y_type == QRC_F32;
-    QRC_CK(w->type == QRC_BF16
-               ? lay_out_and_multiply<__nv_bfloat16>(*w, d_x, m, ldx, d_bias, d_y, ldy, y_float, work, s)
-               : lay_out_and_multiply<__half>(*w, d_x, m, ldx, d_bias, d_y, ldy, y_float, work, s));
-    return QRC_OK;
+    return w->type == QRC_BF16 ? launch_matvec<__nv_bfloat16>(*w, d_x, m, ldx, d_bias, d_y, ldy, y_float, sms, s)
+                               : launch_matvec<__half>(*w, d_x, m, ldx, d_bias, d_y, ldy, y_float, sms, s);
 }

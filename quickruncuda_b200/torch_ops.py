@@ -192,7 +192,7 @@ def dequant_w4(packed: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch
 
 @dequant_w4.register_fake
 def _(packed, scales, zeros, k: int, group: int, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    return scales.new_empty((packed.shape[0], k), dtype=scales.dtype if dtype is None else dtype)
+    return scales.new_empty((scales.shape[1], k), dtype=scales.dtype if dtype is None else dtype)
 
 
 @torch.library.custom_op("qrc::matvec_w4", mutates_args=(), device_types="cuda")
@@ -205,4 +205,4 @@ def matvec_w4(x: torch.Tensor, packed: torch.Tensor, scales: torch.Tensor, zeros
 
 @matvec_w4.register_fake
 def _(x, packed, scales, zeros, group: int, bias=None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
-    return x.new_empty(x.shape[:-1] + (packed.shape[0],), dtype=x.dtype if out_dtype is None else out_dtype)
+    return x.new_empty(x.shape[:-1] + (scales.shape[1],), dtype=x.dtype if out_dtype is None else out_dtype)

@@ -49,13 +49,15 @@ def _check_group(group: int) -> int:
 
 
 def packed_shape(n: int, k: int):
-    return (n, -(-k // 128) * 16)
+    """Tiles of 16 rows by 128 columns, 256 words each."""
+    return (-(-n // 16), -(-k // 128), 256)
 
 
 class Weight4:
     """A 4-bit weight matrix of n rows (outputs) and k columns (inputs).
 
-    packed  int32 [n, ceil(k / 128) * 16], codes in the order of qrc_b200.h
+    packed  int32 [ceil(n / 16), ceil(k / 128), 256], codes in the order of
+            qrc_b200.h
     scales  bfloat16 or float16 [ceil(k / group), n]
     zeros   uint8 [ceil(k / group), n] of 0..15, or None: all 8
 
@@ -66,10 +68,12 @@ class Weight4:
         group, k = _check_group(group), int(k)
         if k < 0:
             raise RuntimeError(f"Weight4: k has to be 0 or more, got {k}")
-        n = int(packed.shape[0]) if packed.dim() else 0
-        _check(packed, "packed", (torch.int32,), packed_shape(n, k))
+        if scales.dim() != 2:
+            raise RuntimeError(f"Weight4: scales have to be 2-D, got {tuple(scales.shape)}")
+        n = int(scales.shape[1])
         groups = (-(-k // group), n)
-        _check(scales, "scales", _TYPES, groups, packed.device)
+        _check(scales, "scales", _TYPES, groups)
+        _check(packed, "packed", (torch.int32,), packed_shape(n, k), scales.device)
         if zeros is not None:
             _check(zeros, "zeros", (torch.uint8,), groups, packed.device)
         for name, t in (("packed", packed), ("scales", scales), ("zeros", zeros)):
@@ -139,13 +143,10 @@ class Weight4:
         x2 = _as_rows(x, m, k, "x")
         y2 = _as_rows(out, m, n, "out")
         ldx, ldy = _pitch(x2, "x"), _pitch(y2, "out")
-        need = self.lib.qrc_w4_matvec_workspace(self._ref, x.data_ptr(), m, ldx)
-        work = _empty(need, torch.uint8, self.device, stream) if need else None
         nat.check(self.lib, "qrc_w4_matvec",
                   self.lib.qrc_w4_matvec(self.device.index, self._ref, x.data_ptr(), m, ldx,
                                          None if bias is None else bias.data_ptr(), out.data_ptr(), ldy,
-                                         _OUT_TYPES[kind], None if work is None else work.data_ptr(),
-                                         _stream_handle(stream, self.device.index) or None))
+                                         _OUT_TYPES[kind], _stream_handle(stream, self.device.index) or None))
         return out
 
 

@@ -1,6 +1,7 @@
 """4-bit weights (quickruncuda_b200/weight4.py, qrc_w4_*) without a GPU: what
 is refused before any GPU work, and the shapes of the operators."""
 import ctypes
+import math
 
 import pytest
 import torch
@@ -11,7 +12,7 @@ from quickruncuda_b200 import _native as nat
 from quickruncuda_b200.weight4 import packed_shape
 from torch._subclasses.fake_tensor import FakeTensorMode
 
-P, S, Z, X, Y, W = (i << 24 for i in range(1, 7))       # addresses far apart, never read
+P, S, Z, X, Y = (i << 24 for i in range(1, 6))       # addresses far apart, never read
 
 
 def _w4(packed=P, scales=S, zeros=None, n=48, k=300, group=128, type=nat.TYPE_BF16):
@@ -20,23 +21,22 @@ def _w4(packed=P, scales=S, zeros=None, n=48, k=300, group=128, type=nat.TYPE_BF
 
 def test_words(lib):
     assert lib.qrc_w4_words(0, 5) == 0 and lib.qrc_w4_words(5, 0) == 0
-    assert lib.qrc_w4_words(3, 1) == 48 and lib.qrc_w4_words(3, 128) == 48 and lib.qrc_w4_words(3, 129) == 96
+    assert lib.qrc_w4_words(3, 1) == 256 and lib.qrc_w4_words(16, 128) == 256 and lib.qrc_w4_words(17, 129) == 1024
     for k in (0, 1, 127, 128, 129, 1000):
-        n, words = packed_shape(7, k)
-        assert n * words == lib.qrc_w4_words(7, k)
+        for n in (0, 1, 16, 17):
+            assert math.prod(packed_shape(n, k)) == lib.qrc_w4_words(n, k)
 
 
 @pytest.mark.parametrize("bad", [dict(group=96), dict(group=16), dict(group=0), dict(group=512), dict(type=nat.TYPE_F32),
                                  dict(type=7), dict(packed=None), dict(packed=P + 4), dict(scales=None),
-                                 dict(scales=S + 1), dict(n=(1 << 31) + 1), dict(k=(1 << 31) + 1)])
+                                 dict(scales=S + 1), dict(n=1 << 31), dict(k=1 << 31)])
 def test_bad_matrices_are_refused(lib, bad):
     w = _w4(**bad)
     k = max(300, bad.get("k", 0))
     assert lib.qrc_w4_quant(0, X, k, 1, w, None) == nat.QRC_ERR_INVALID
     assert lib.qrc_w4_pack(0, X, k, w, None) == nat.QRC_ERR_INVALID
     assert lib.qrc_w4_dequant(0, w, Y, k, nat.TYPE_F32, None) == nat.QRC_ERR_INVALID
-    assert lib.qrc_w4_matvec(0, w, X, 1, k, None, Y, 48, nat.TYPE_F32, None, None) == nat.QRC_ERR_INVALID
-    assert lib.qrc_w4_matvec_workspace(w, X + 2, 1, k) == 0
+    assert lib.qrc_w4_matvec(0, w, X, 1, k, None, Y, 48, nat.TYPE_F32, None) == nat.QRC_ERR_INVALID
 
 
 def test_bad_arguments_are_refused(lib):
@@ -55,20 +55,11 @@ def test_bad_arguments_are_refused(lib):
     assert lib.qrc_w4_dequant(0, _w4(), Y + 2, 300, 0, None) == bad
     assert lib.qrc_w4_dequant(0, _w4(), Y, 299, 0, None) == bad
     assert lib.qrc_w4_dequant(0, _w4(), P + 64, 300, 0, None) == bad
-    ok = dict(device=0, w=_w4(), x=X, m=2, ldx=304, bias=None, y=Y, ldy=48, type=nat.TYPE_BF16, work=None, stream=None)
+    ok = dict(device=0, w=_w4(), x=X, m=2, ldx=304, bias=None, y=Y, ldy=48, type=nat.TYPE_BF16, stream=None)
     for change in (dict(x=None), dict(y=None), dict(x=X + 1), dict(bias=X + 1), dict(y=Y + 1), dict(ldx=299), dict(ldy=47),
-                   dict(type=nat.TYPE_F16), dict(type=5), dict(y=Y + 2, type=nat.TYPE_F32), dict(m=(1 << 31) + 1),
-                   dict(y=X + 64), dict(y=P), dict(y=S), dict(bias=Y), dict(x=X + 2), dict(x=X, ldx=301),
-                   dict(x=X, ldx=301, work=W + 8)):
+                   dict(type=nat.TYPE_F16), dict(type=5), dict(y=Y + 2, type=nat.TYPE_F32), dict(m=1 << 31),
+                   dict(y=X + 64), dict(y=P), dict(y=S), dict(bias=Y)):
         assert lib.qrc_w4_matvec(*dict(ok, **change).values()) == bad, change
-
-
-def test_workspace(lib):
-    assert lib.qrc_w4_matvec_workspace(_w4(), X, 1, 300) == 0                  # one row, aligned
-    assert lib.qrc_w4_matvec_workspace(_w4(), X, 2, 304) == 0
-    assert lib.qrc_w4_matvec_workspace(_w4(), X, 2, 300) == 2 * 384 * 2
-    assert lib.qrc_w4_matvec_workspace(_w4(), X + 2, 1, 300) == 384 * 2
-    assert lib.qrc_w4_matvec_workspace(_w4(), X + 2, 0, 300) == 0
 
 
 def test_python_refusals():
@@ -82,10 +73,10 @@ def test_python_refusals():
                 q.quant_w4(bad)
         with pytest.raises(RuntimeError, match="group"):
             q.quant_w4(w, group=100)
-        packed = torch.empty(48, 48, device="cuda", dtype=torch.int32)
+        packed = torch.empty(3, 3, 256, device="cuda", dtype=torch.int32)
         scales = torch.empty(3, 48, device="cuda", dtype=torch.bfloat16)
         zeros = torch.empty(3, 48, device="cuda", dtype=torch.uint8)
-        for change, what in (((packed.float(), scales, zeros, 300, 128), "packed"), ((packed, scales, zeros, 400, 128), "packed"),
+        for change, what in (((packed.float(), scales, zeros, 300, 128), "packed"), ((packed[:, :2], scales, zeros, 300, 128), "packed"), ((packed, scales, zeros, 400, 128), "scales"),
                              ((packed, scales.float(), zeros, 300, 128), "scales"), ((packed, scales, zeros, 300, 64), "scales"),
                              ((packed, scales, zeros.int(), 300, 128), "zeros"), ((packed, scales, zeros[:2], 300, 128), "zeros"),
                              ((packed, torch.empty(48, 3, device="cuda", dtype=torch.bfloat16).t(), None, 300, 128), "contiguous"),
@@ -100,7 +91,7 @@ def test_operator_shapes():
     with FakeTensorMode():
         w = torch.empty(48, 300, device="cuda", dtype=torch.float16)
         packed, scales, zeros = torch.ops.qrc.quant_w4(w, 64, False)
-        assert packed.shape == (48, 48) and packed.dtype == torch.int32
+        assert packed.shape == (3, 3, 256) and packed.dtype == torch.int32
         assert scales.shape == (5, 48) == zeros.shape and scales.dtype == torch.float16 and zeros.dtype == torch.uint8
         assert torch.ops.qrc.quant_w4(w)[2].numel() == 0
         v = torch.ops.qrc.dequant_w4(packed, scales, zeros, 300, 64)

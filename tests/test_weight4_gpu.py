@@ -17,15 +17,17 @@ def _type(name):
     return {"bf16": torch.bfloat16, "f16": torch.float16}[name]
 
 
-def _unpack(packed, k):
+def _unpack(packed, n, k):
     """Codes [n, k] from the layout that qrc_b200.h describes."""
     import torch
-    n = packed.shape[0]
-    words = packed.view(n, -1, 4, 4).long() & 0xFFFFFFFF                 # [n, block, t, j]
-    codes = torch.empty(n, words.shape[1], 4, 4, 8, dtype=torch.uint8, device=packed.device)   # [n, block, j, t, e]
+    a, b, _ = packed.shape
+    words = packed.view(a, b, 16, 4, 4).long() & 0xFFFFFFFF             # [tile row, tile, row, t, j]
+    codes = torch.empty(a, 16, b, 4, 4, 8, dtype=torch.uint8, device=packed.device)     # [.., row, tile, j, t, e]
     for e in range(8):
-        codes[..., e] = (words >> ((e // 2) * 4 + (e % 2) * 16) & 15).transpose(2, 3).to(torch.uint8)
-    return codes.reshape(n, -1)[:, :k]
+        at = (3 + e // 2 * 4 + e % 2 * 16) % 32
+        rotated = (words >> at | words << (32 - at)) & 15
+        codes[..., e] = rotated.permute(0, 2, 1, 4, 3).to(torch.uint8)
+    return codes.view(a * 16, b * 128)[:n, :k]
 
 
 def _round16(v, kind):
@@ -67,7 +69,7 @@ def _check_quant(qrc, w, group, symmetric):
     assert (w4.zeros is None) == symmetric
     if not symmetric:
         assert torch.equal(w4.zeros, zeros)
-    got = _unpack(w4.packed, w.shape[1])
+    got = _unpack(w4.packed, *w.shape)
     bad = got != codes
     assert not bad.any(), (got[bad][:5], codes[bad][:5], w[bad][:5])
     # the values, exact in float32 and rounded once in 16 bits, within the
@@ -190,7 +192,7 @@ def test_matvec_shapes(cuda, qrc, kind, group, symmetric):
     for i, (n, k) in enumerate(MATVEC_SHAPES):
         codes, scales, zeros, gen = _case(cuda, n, k, kind, group, symmetric, seed=i)
         w4 = qrc.Weight4.from_codes(codes, scales, zeros, group=group)
-        assert torch.equal(_unpack(w4.packed, k), codes)
+        assert torch.equal(_unpack(w4.packed, n, k), codes)
         values = _values(codes, scales, zeros, group)
         for m in (1, 2, 3, 7, 8, 9, 16, 17, 32, 33, 70) if i % 4 == 0 else (1, 5, 13, 31):
             x = torch.randn(m, k, generator=gen, device=cuda).to(_type(kind))
