@@ -1,0 +1,28 @@
+"""Streams and allocations of calls that torch's allocator serves."""
+from __future__ import annotations
+
+import torch
+
+# torch.cuda.current_stream builds a Stream object for each call, half the
+# host time of a small launch; the raw handle is what is needed.
+_raw_current = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def stream_handle(stream, device: int):
+    """The cudaStream_t a call runs on, None for the legacy default stream."""
+    if stream is None:
+        if _raw_current is not None:
+            return _raw_current(device) or None
+        return torch.cuda.current_stream(device).cuda_stream or None
+    return (stream if isinstance(stream, int) else int(stream.cuda_stream)) or None
+
+
+def empty(shape, dtype, device, stream) -> torch.Tensor:
+    """torch.empty that belongs to the stream the call runs on, so that its
+    memory is not handed out again before the call is done."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)

@@ -41,18 +41,6 @@ def _stream_handle(stream, device: int) -> int:
     return int(stream.cuda_stream)
 
 
-def _empty(shape, dtype, device, stream):
-    """torch.empty that belongs to the stream the call runs on, so that its
-    memory is not handed out again before the call is done."""
-    import torch
-    if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    if isinstance(stream, int):
-        stream = torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
-    with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
-
-
 def _nbytes(x) -> int:
     if hasattr(x, "untyped_storage"):
         return int(x.numel() * x.element_size())

@@ -2,6 +2,7 @@
 #pragma once
 
 #include <cuda_runtime.h>
+#include <atomic>
 #include <cstdint>
 #include <map>
 #include <mutex>
@@ -38,11 +39,18 @@ struct DeviceScope {
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 // SMs of `dev`, or 0 when there is no such device or it is not an sm_100 one.
+// Asked once per device: a device's properties do not change.
 inline int sm100_sms(int dev) {
-    int ndev = 0, major = 0, sms = 0;
-    if (cudaGetDeviceCount(&ndev) != cudaSuccess || dev < 0 || dev >= ndev) return 0;
+    constexpr int kMaxDevices = 64;
+    static std::atomic<int> known[kMaxDevices];
+    if (dev < 0 || dev >= kMaxDevices) return 0;
+    int sms = known[dev].load(std::memory_order_relaxed);
+    if (sms) return sms;
+    int ndev = 0, major = 0;
+    if (cudaGetDeviceCount(&ndev) != cudaSuccess || dev >= ndev) return 0;
     if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess || major != 10) return 0;
     if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    known[dev].store(sms, std::memory_order_relaxed);
     return sms;
 }
 

@@ -10,6 +10,8 @@
 // norm adds the partials in a fixed order, so results do not change from run
 // to run and no counter has to be zeroed.  The list of tensors travels in the
 // kernel's parameters, so a captured launch carries its own copy.
+#define QRC_NO_PLUGIN_ABI
+#include "side_aware_b200.cu"
 #include "qrc_host.h"
 #include "../../include/qrc_b200.h"
 
@@ -25,8 +27,25 @@
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kMaxBlocks = 2368;              // 16 blocks per SM: what SMs differ in speed evens out
-constexpr int kMinChunkLog2 = 12, kMaxChunkLog2 = 15;
+// Blocks.  The norm reads fastest with one wave of two blocks per SM (128 MiB
+// of bf16: 24.5 us with 2, 26.1 with 4, 28.7 with 8 blocks per SM, 41.5 with
+// 32); the scale pass, which writes too, with a block per 256 KiB of input up
+// to 64 per SM (2 GB: 926 us for norm and scale, 1020 with two per SM).
+constexpr uint32_t kNormBlocksPerSm = 2, kScaleBlocksPerSm = 64;
+constexpr uint64_t kScaleBytes = 256 << 10;
+// Up to this much input the second read finds most of it in L2 (126 MB), as
+// long as what is read or written for the last time does not stay there:
+// streaming loads and stores. 64 MiB into another tensor: 35.0 us with, 38.9
+// without; 512 MiB: 256 with, 248 without.
+constexpr uint64_t kStreamBytes = 192ull << 20;
+constexpr uint32_t kFold = 1024;              // partial results that every block of the scale pass adds up itself
+constexpr int kMinChunkLog2 = 10, kMaxChunkLog2 = 15;
+// Up to this much input one cluster of blocks does everything in one launch: a
+// call takes 6 us of host time instead of 9.5 (norm) or 9.5 to 12 (clip), and
+// on the GPU about as long as two (256 KiB: norm 3.6 us, two launches 3.8).
+// Above it the eight SMs are what bounds it (1 MiB: 5.6 us, two launches 4.5).
+constexpr int kCluster = 8, kSmallThreads = 256;
+constexpr uint64_t kSmallBytes = 512 << 10;
 constexpr int kKindShift = 56;                // n_kind: elements, input type << 56, output type << 60
 
 // One tensor: `n` elements at in and out.  cols == 0: dense; else rows of
@@ -50,9 +69,6 @@ struct Table {
     uint32_t count, chunks, chunk_log2, first_partial;
 };
 static_assert(sizeof(Table<kLargeTable>) + 32 <= 32764, "kernel parameter limit");
-
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 __device__ __forceinline__ uint4 load_once(const uint4* p) {
     uint4 v;
@@ -128,10 +144,15 @@ struct Acc<QRC_NORM_INF> {
     uint32_t m = 0;
     __device__ __forceinline__ void one(float x) { m = max(m, __float_as_uint(x) & 0x7fffffffu); }
     template <class T> __device__ __forceinline__ void vec(const uint4& v) {
-        float f[16 / sizeof(T)];
-        unpack<T>(v, f);
-#pragma unroll
-        for (int i = 0; i < 16 / (int)sizeof(T); i++) one(f[i]);
+        if (sizeof(T) == 4) {
+            m = max(max(max(m, v.x & 0x7fffffffu), max(v.y & 0x7fffffffu, v.z & 0x7fffffffu)), v.w & 0x7fffffffu);
+            return;
+        }
+        // Magnitudes of 16-bit types order like whole numbers, two at a time.
+        constexpr uint32_t kMask = 0x7fff7fffu;
+        const uint32_t p = __vmaxu2(__vmaxu2(v.x & kMask, v.y & kMask), __vmaxu2(v.z & kMask, v.w & kMask));
+        const uint16_t h = (uint16_t)max(p >> 16, p & 0xffffu);
+        one(to_float(reinterpret_cast<const T&>(h)));
     }
     __device__ __forceinline__ double value() const { return (double)__uint_as_float(m); }
 };
@@ -143,8 +164,8 @@ template <int NORM> __device__ __forceinline__ double combine(double x, double y
 }
 
 // The combination of every thread's value, in a fixed order, in all threads.
-template <int NORM> __device__ __forceinline__ double block_combine(double v) {
-    __shared__ double s_part[kThreads / 32];
+template <int NORM, int THREADS = kThreads> __device__ __forceinline__ double block_combine(double v) {
+    __shared__ double s_part[THREADS / 32];
     __shared__ double s_all;
 #pragma unroll
     for (int d = 16; d; d >>= 1) v = combine<NORM>(v, __shfl_xor_sync(0xffffffffu, v, d));
@@ -153,7 +174,7 @@ template <int NORM> __device__ __forceinline__ double block_combine(double v) {
     if (threadIdx.x == 0) {
         double t = s_part[0];
 #pragma unroll
-        for (int i = 1; i < kThreads / 32; i++) t = combine<NORM>(t, s_part[i]);
+        for (int i = 1; i < THREADS / 32; i++) t = combine<NORM>(t, s_part[i]);
         s_all = t;
     }
     __syncthreads();
@@ -193,60 +214,69 @@ __device__ __forceinline__ void for_share(const Table<CAP>& t, uint32_t block, u
 
 // -- norm ----------------------------------------------------------------------
 
-template <class T, class A>
+// The threads that share a part of a tensor: a block, or a warp.
+template <int SIZE> struct Team {
+    static constexpr uint32_t kSize = SIZE;
+    static __device__ __forceinline__ uint32_t rank() { return threadIdx.x % SIZE; }
+};
+
+template <class G, class T, class A>
 __device__ __forceinline__ void norm_dense(const T* p, uint64_t n, A& acc) {
-    constexpr int VE = 16 / sizeof(T), U = 4;
+    constexpr int VE = 16 / sizeof(T), U = G::kSize == 32 ? 8 : 4;
     const uint64_t lead = ((16 - ((uintptr_t)p & 15)) & 15) / sizeof(T);
     const uint32_t head = (uint32_t)min(n, lead);
-    if (threadIdx.x < head) acc.one(to_float(p[threadIdx.x]));
+    if (G::rank() < head) acc.one(to_float(p[G::rank()]));
     p += head;
     n -= head;
     const uint4* v = reinterpret_cast<const uint4*>(p);
     const uint32_t nv = (uint32_t)(n / VE);
-    uint32_t i = threadIdx.x;
-    for (; i + (U - 1) * kThreads < nv; i += U * kThreads) {
+    uint32_t i = G::rank();
+    for (; i + (U - 1) * G::kSize < nv; i += U * G::kSize) {
         uint4 r[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) r[u] = load_once(v + i + u * kThreads);
+        for (int u = 0; u < U; u++) r[u] = load_once(v + i + u * G::kSize);
 #pragma unroll
         for (int u = 0; u < U; u++) acc.template vec<T>(r[u]);
     }
-    for (; i < nv; i += kThreads) acc.template vec<T>(load_once(v + i));
+    for (; i < nv; i += G::kSize) acc.template vec<T>(load_once(v + i));
     const uint32_t tail = (uint32_t)(n - (uint64_t)nv * VE);
-    if (threadIdx.x < tail) acc.one(to_float(p[(uint64_t)nv * VE + threadIdx.x]));
+    if (G::rank() < tail) acc.one(to_float(p[(uint64_t)nv * VE + G::rank()]));
 }
 
-template <class T, class A>
+template <class G, class T, class A>
 __device__ __forceinline__ void norm_pitched(const Entry& e, uint64_t e0, uint64_t e1, A& acc) {
     const T* p = static_cast<const T*>(e.in);
     const uint64_t row = e0 / e.cols;
     const uint32_t col = (uint32_t)(e0 - row * e.cols), count = (uint32_t)(e1 - e0);
     p += row * e.in_pitch;
-    for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
+    for (uint32_t i = G::rank(); i < count; i += G::kSize) {
         const uint32_t at = col + i, r = at / e.cols;
         acc.one(to_float(p[(uint64_t)r * e.in_pitch + (at - r * e.cols)]));
     }
 }
 
-template <class T, class A>
+template <class G, class T, class A>
 __device__ __forceinline__ void norm_part(const Entry& e, uint64_t e0, uint64_t e1, A& acc) {
-    if (e.cols) norm_pitched<T>(e, e0, e1, acc);
-    else norm_dense(static_cast<const T*>(e.in) + e0, e1 - e0, acc);
+    if (e.cols) norm_pitched<G, T>(e, e0, e1, acc);
+    else norm_dense<G>(static_cast<const T*>(e.in) + e0, e1 - e0, acc);
+}
+
+template <class G, int NORM>
+__device__ __forceinline__ void norm_entry(const Entry& e, uint64_t e0, uint64_t e1, Acc<NORM>& acc) {
+    switch ((e.n_kind >> kKindShift) & 15) {
+        case QRC_F32: norm_part<G, float>(e, e0, e1, acc); break;
+        case QRC_BF16: norm_part<G, __nv_bfloat16>(e, e0, e1, acc); break;
+        default: norm_part<G, __half>(e, e0, e1, acc); break;
+    }
 }
 
 template <int NORM, int CAP>
 __global__ void __launch_bounds__(kThreads)
 qrc_k_list_norm(const __grid_constant__ Table<CAP> t, double* partials) {
-    wait_for_previous();
-    let_next_start();
+    qrc::griddep_wait();
+    qrc::griddep_launch_dependents();
     Acc<NORM> acc;
-    for_share(t, blockIdx.x, gridDim.x, [&](const Entry& e, uint64_t e0, uint64_t e1) {
-        switch ((e.n_kind >> kKindShift) & 15) {
-            case QRC_F32: norm_part<float>(e, e0, e1, acc); break;
-            case QRC_BF16: norm_part<__nv_bfloat16>(e, e0, e1, acc); break;
-            default: norm_part<__half>(e, e0, e1, acc); break;
-        }
-    });
+    for_share(t, blockIdx.x, gridDim.x, [&](const Entry& e, uint64_t e0, uint64_t e1) { norm_entry<Team<kThreads>>(e, e0, e1, acc); });
     const double v = block_combine<NORM>(acc.value());
     if (threadIdx.x == 0) partials[t.first_partial + blockIdx.x] = v;
 }
@@ -262,8 +292,8 @@ template <int NORM> __device__ __forceinline__ double total_norm(const double* p
 template <int NORM>
 __global__ void __launch_bounds__(kThreads)
 qrc_k_list_finish(double* work, uint32_t count, float* norm) {
-    wait_for_previous();
-    let_next_start();
+    qrc::griddep_wait();
+    qrc::griddep_launch_dependents();
     const double v = total_norm<NORM>(work + 1, count);
     if (threadIdx.x == 0) {
         work[0] = v;
@@ -280,7 +310,7 @@ __device__ __forceinline__ float clip_factor(double norm, double max_norm) {
     return k >= 1.0 ? 1.0f : (float)k;
 }
 
-template <class TI, class TO>
+template <bool STREAM, class TI, class TO>
 __device__ __forceinline__ void scale_vec(const uint4& v, void* out, float k) {
     constexpr int VE = 16 / sizeof(TI), OB = VE * sizeof(TO);
     float f[VE];
@@ -288,84 +318,147 @@ __device__ __forceinline__ void scale_vec(const uint4& v, void* out, float k) {
     __align__(16) TO r[VE];
 #pragma unroll
     for (int i = 0; i < VE; i++) r[i] = from_float<TO>(f[i] * k);
+    const uint4* w = reinterpret_cast<const uint4*>(r);
     if (OB == 8) *reinterpret_cast<uint2*>(out) = *reinterpret_cast<const uint2*>(r);
-    else {
-#pragma unroll
-        for (int i = 0; i < OB / 16; i++) reinterpret_cast<uint4*>(out)[i] = reinterpret_cast<const uint4*>(r)[i];
+    else if (OB == 16) {
+        if (STREAM) __stcs(reinterpret_cast<uint4*>(out), w[0]);
+        else *reinterpret_cast<uint4*>(out) = w[0];
+    } else {
+        // A whole 32-byte sector per thread: with two stores of 16 bytes, each
+        // filling half of every sector, 1.36 GB of bf16 into float32 took 917
+        // us (norm included) instead of 828.
+        asm volatile("st.global.L1::no_allocate.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                     :: "l"(out), "r"(w[0].x), "r"(w[0].y), "r"(w[0].z), "r"(w[0].w), "r"(w[1].x), "r"(w[1].y),
+                     "r"(w[1].z), "r"(w[1].w) : "memory");
     }
 }
 
-template <class TI, class TO>
+template <class G, bool STREAM, class TI, class TO>
 __device__ __forceinline__ void scale_dense(const TI* p, TO* q, uint64_t n, float k) {
-    constexpr int VE = 16 / sizeof(TI), OB = VE * (int)sizeof(TO), OA = OB < 16 ? OB : 16, U = 4;
+    constexpr int VE = 16 / sizeof(TI), OB = VE * (int)sizeof(TO), U = 4;
     const uint64_t lead = ((16 - ((uintptr_t)p & 15)) & 15) / sizeof(TI);
     const uint32_t head = (uint32_t)min(n, lead);
     // Vectors need both sides aligned after the same number of elements;
     // otherwise every element goes by itself.
-    if (((uintptr_t)(q + head) & (OA - 1)) != 0) {
-        for (uint64_t i = threadIdx.x; i < n; i += kThreads) q[i] = from_float<TO>(to_float(p[i]) * k);
+    if (((uintptr_t)(q + head) & (OB - 1)) != 0) {
+        for (uint64_t i = G::rank(); i < n; i += G::kSize) q[i] = from_float<TO>(to_float(p[i]) * k);
         return;
     }
-    if (threadIdx.x < head) q[threadIdx.x] = from_float<TO>(to_float(p[threadIdx.x]) * k);
+    if (G::rank() < head) q[G::rank()] = from_float<TO>(to_float(p[G::rank()]) * k);
     p += head;
     q += head;
     n -= head;
     const uint4* v = reinterpret_cast<const uint4*>(p);
     const uint32_t nv = (uint32_t)(n / VE);
-    uint32_t i = threadIdx.x;
-    for (; i + (U - 1) * kThreads < nv; i += U * kThreads) {
+    uint32_t i = G::rank();
+    for (; i + (U - 1) * G::kSize < nv; i += U * G::kSize) {
         uint4 r[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) r[u] = v[i + u * kThreads];
+        for (int u = 0; u < U; u++) r[u] = (STREAM ? __ldcs(v + i + u * G::kSize) : v[i + u * G::kSize]);
 #pragma unroll
-        for (int u = 0; u < U; u++) scale_vec<TI, TO>(r[u], q + (uint64_t)(i + u * kThreads) * VE, k);
+        for (int u = 0; u < U; u++) scale_vec<STREAM, TI, TO>(r[u], q + (uint64_t)(i + u * G::kSize) * VE, k);
     }
-    for (; i < nv; i += kThreads) scale_vec<TI, TO>(v[i], q + (uint64_t)i * VE, k);
+    for (; i < nv; i += G::kSize) scale_vec<STREAM, TI, TO>(STREAM ? __ldcs(v + i) : v[i], q + (uint64_t)i * VE, k);
     const uint64_t done = (uint64_t)nv * VE;
-    if (threadIdx.x < (uint32_t)(n - done)) q[done + threadIdx.x] = from_float<TO>(to_float(p[done + threadIdx.x]) * k);
+    if (G::rank() < (uint32_t)(n - done)) q[done + G::rank()] = from_float<TO>(to_float(p[done + G::rank()]) * k);
 }
 
-template <class TI, class TO>
+template <class G, bool STREAM, class TI, class TO>
 __device__ __forceinline__ void scale_part(const Entry& e, uint64_t e0, uint64_t e1, float k) {
     const TI* p = static_cast<const TI*>(e.in);
     TO* q = static_cast<TO*>(e.out);
-    if (!e.cols) return scale_dense(p + e0, q + e0, e1 - e0, k);
+    if (!e.cols) return scale_dense<G, STREAM>(p + e0, q + e0, e1 - e0, k);
     const uint64_t row = e0 / e.cols;
     const uint32_t col = (uint32_t)(e0 - row * e.cols), count = (uint32_t)(e1 - e0);
     p += row * e.in_pitch;
     q += row * e.out_pitch;
-    for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
+    for (uint32_t i = G::rank(); i < count; i += G::kSize) {
         const uint32_t at = col + i, r = at / e.cols, c = at - r * e.cols;
         q[(uint64_t)r * e.out_pitch + c] = from_float<TO>(to_float(p[(uint64_t)r * e.in_pitch + c]) * k);
     }
 }
 
-template <class TI>
+template <class G, bool STREAM, class TI>
 __device__ __forceinline__ void scale_from(const Entry& e, uint64_t e0, uint64_t e1, float k) {
     switch (e.n_kind >> (kKindShift + 4)) {
-        case QRC_F32: scale_part<TI, float>(e, e0, e1, k); break;
-        case QRC_BF16: scale_part<TI, __nv_bfloat16>(e, e0, e1, k); break;
-        default: scale_part<TI, __half>(e, e0, e1, k); break;
+        case QRC_F32: scale_part<G, STREAM, TI, float>(e, e0, e1, k); break;
+        case QRC_BF16: scale_part<G, STREAM, TI, __nv_bfloat16>(e, e0, e1, k); break;
+        default: scale_part<G, STREAM, TI, __half>(e, e0, e1, k); break;
     }
 }
 
-// `given` (a float norm in device memory) or work[0] decides the factor.  The
+template <class G, bool STREAM>
+__device__ __forceinline__ void scale_entry(const Entry& e, uint64_t e0, uint64_t e1, float k) {
+    const int from = (int)(e.n_kind >> kKindShift) & 15, to = (int)(e.n_kind >> (kKindShift + 4));
+    if (k == 1.0f && e.in == e.out && from == to) return;           // x * 1 is what is there already
+    switch (from) {
+        case QRC_F32: scale_from<G, STREAM, float>(e, e0, e1, k); break;
+        case QRC_BF16: scale_from<G, STREAM, __nv_bfloat16>(e, e0, e1, k); break;
+        default: scale_from<G, STREAM, __half>(e, e0, e1, k); break;
+    }
+}
+
+// `given` (a float norm in device memory) decides the factor; or work[0]; or,
+// with `count` partial results of that norm in the workspace, their total,
+// which every block adds up for itself and the first one publishes.  The
 // blocks walk the list from its end, which the norm pass read last.
-template <int CAP>
+template <int CAP, bool STREAM>
 __global__ void __launch_bounds__(kThreads)
-qrc_k_list_scale(const __grid_constant__ Table<CAP> t, const double* work, const float* given, double max_norm) {
-    wait_for_previous();
-    let_next_start();
-    const float k = clip_factor(given ? (double)*given : work[0], max_norm);
-    for_share(t, gridDim.x - 1 - blockIdx.x, gridDim.x, [&](const Entry& e, uint64_t e0, uint64_t e1) {
-        const int from = (int)(e.n_kind >> kKindShift) & 15, to = (int)(e.n_kind >> (kKindShift + 4));
-        if (k == 1.0f && e.in == e.out && from == to) return;       // x * 1 is what is there already
-        switch (from) {
-            case QRC_F32: scale_from<float>(e, e0, e1, k); break;
-            case QRC_BF16: scale_from<__nv_bfloat16>(e, e0, e1, k); break;
-            default: scale_from<__half>(e, e0, e1, k); break;
-        }
-    });
+qrc_k_list_scale(const __grid_constant__ Table<CAP> t, const double* work, const float* given, double max_norm,
+                 int norm, uint32_t count, float* norm_out) {
+    qrc::griddep_wait();
+    qrc::griddep_launch_dependents();
+    double v;
+    if (given) v = (double)*given;
+    else if (!count) v = work[0];
+    else {
+        v = norm == QRC_NORM_1 ? total_norm<QRC_NORM_1>(work + 1, count)
+            : norm == QRC_NORM_2 ? total_norm<QRC_NORM_2>(work + 1, count) : total_norm<QRC_NORM_INF>(work + 1, count);
+        if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)v;
+    }
+    const float k = clip_factor(v, max_norm);
+    for_share(t, gridDim.x - 1 - blockIdx.x, gridDim.x,
+              [&](const Entry& e, uint64_t e0, uint64_t e1) { scale_entry<Team<kThreads>, STREAM>(e, e0, e1, k); });
+}
+
+// -- short lists: one cluster does it all ----------------------------------------
+
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Norm, and with `clip` scaling, in one launch of one cluster: the blocks
+// exchange their partial results through distributed shared memory, so there
+// is no workspace and no second launch.  Every warp takes chunks of its own,
+// so short tensors do not wait for one another.
+template <int NORM, int CAP>
+__global__ void __launch_bounds__(kSmallThreads)
+qrc_k_list_small(const __grid_constant__ Table<CAP> t, float* norm, int clip, double max_norm) {
+    __shared__ double s_mine;
+    qrc::griddep_wait();
+    qrc::griddep_launch_dependents();
+    const uint32_t blocks = gridDim.x, warps = blocks * (kSmallThreads / 32);
+    const uint32_t warp = (threadIdx.x >> 5) * blocks + blockIdx.x;     // neighbours on different SMs
+    Acc<NORM> acc;
+    for_share(t, warp, warps, [&](const Entry& e, uint64_t e0, uint64_t e1) { norm_entry<Team<32>>(e, e0, e1, acc); });
+    const double mine = block_combine<NORM, kSmallThreads>(acc.value());
+    if (threadIdx.x == 0) s_mine = mine;
+    cluster_barrier();
+    double v = 0.0;
+    for (uint32_t i = 0; i < blocks; i++) {
+        uint32_t at;
+        double part;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(&s_mine)), "r"(i));
+        asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(part) : "r"(at) : "memory");
+        v = combine<NORM>(v, part);
+    }
+    if (NORM == QRC_NORM_2) v = sqrt(v);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && norm) *norm = (float)v;
+    if (clip) {
+        const float k = clip_factor(v, max_norm);
+        for_share(t, warp, warps, [&](const Entry& e, uint64_t e0, uint64_t e1) { scale_entry<Team<32>, false>(e, e0, e1, k); });
+    }
+    cluster_barrier();                                              // no block leaves while another reads its part
 }
 
 // ---------------------------------------------------------------------------
@@ -374,7 +467,7 @@ qrc_k_list_scale(const __grid_constant__ Table<CAP> t, const double* work, const
 
 struct Launch {
     std::vector<Entry> entries;
-    uint32_t chunks = 0, grid = 0, first_partial = 0;
+    uint32_t chunks = 0, grid = 0, scale_grid = 0, first_partial = 0;
 };
 
 inline uint64_t elem_bytes(int type) { return type == QRC_F32 ? 4 : 2; }
@@ -436,6 +529,8 @@ bool can_write(const std::vector<qrc_tensor>& ts) {
 struct qrc_list {
     int device = 0;
     bool writable = false;
+    bool small = false;                       // one cluster, no workspace
+    bool stream = false;                      // the scale pass streams
     uint32_t partials = 0, chunk_log2 = kMaxChunkLog2;
     std::vector<Launch> launches;
 };
@@ -447,7 +542,7 @@ void plan(qrc_list& l, const std::vector<qrc_tensor>& ts, int sms) {
     uint64_t total = 0;
     for (const qrc_tensor& t : ts) total += t.rows * t.cols * elem_bytes(t.in_type);
     // Chunks of 32 KiB, smaller ones where they would leave SMs without work.
-    while (l.chunk_log2 > kMinChunkLog2 && (total >> l.chunk_log2) < 2u * sms) l.chunk_log2--;
+    while (l.chunk_log2 > kMinChunkLog2 && (total >> l.chunk_log2) < 4u * sms) l.chunk_log2--;
     for (const qrc_tensor& t : ts) {
         const uint64_t n = t.rows * t.cols;
         const uint64_t per = (1ull << l.chunk_log2) / elem_bytes(t.in_type), chunks = (n + per - 1) / per;
@@ -466,8 +561,12 @@ void plan(qrc_list& l, const std::vector<qrc_tensor>& ts, int sms) {
         a.entries.push_back(e);
         a.chunks += (uint32_t)chunks;
     }
+    l.small = total <= kSmallBytes && l.launches.size() == 1;
+    l.stream = total <= kStreamBytes;
     for (Launch& a : l.launches) {
-        a.grid = std::min<uint32_t>(a.chunks, kMaxBlocks);
+        a.grid = std::min<uint32_t>(a.chunks, kNormBlocksPerSm * sms);
+        const uint64_t blocks = std::max<uint64_t>(total / kScaleBytes, kNormBlocksPerSm * sms);
+        a.scale_grid = (uint32_t)std::min<uint64_t>(std::min<uint64_t>(a.chunks, blocks), kScaleBlocksPerSm * sms);
         a.first_partial = l.partials;
         l.partials += a.grid;
     }
@@ -489,29 +588,53 @@ cudaError_t launch_norm(const qrc_list& l, const Launch& a, double* work, cudaSt
     return launch_overlapped(qrc_k_list_norm<NORM, CAP>, dim3(a.grid), kThreads, 0, s, 1, t, work + 1);
 }
 
-template <int CAP>
-cudaError_t launch_scale(const qrc_list& l, const Launch& a, const double* work, const float* given, double max_norm,
-                         cudaStream_t s) {
+template <int NORM, int CAP>
+cudaError_t launch_small(const qrc_list& l, float* norm, int clip, double max_norm, cudaStream_t s) {
+    const Launch& a = l.launches[0];
     Table<CAP> t;
     fill_table(t, l, a);
-    return launch_overlapped(qrc_k_list_scale<CAP>, dim3(a.grid), kThreads, 0, s, 1, t, work, given, max_norm);
+    return launch_overlapped(qrc_k_list_small<NORM, CAP>, dim3(kCluster), kSmallThreads, 0, s, kCluster, t, norm, clip, max_norm);
+}
+
+template <int CAP>
+cudaError_t launch_scale(const qrc_list& l, const Launch& a, const double* work, const float* given, double max_norm,
+                         int norm, uint32_t count, float* norm_out, cudaStream_t s) {
+    Table<CAP> t;
+    fill_table(t, l, a);
+    return launch_overlapped(l.stream ? qrc_k_list_scale<CAP, true> : qrc_k_list_scale<CAP, false>, dim3(a.scale_grid),
+                             kThreads, 0, s, 1, t, work, given, max_norm, norm, count, norm_out);
 }
 
 template <int NORM>
-cudaError_t run_norm(const qrc_list& l, double* work, float* norm, cudaStream_t s) {
+cudaError_t run_small(const qrc_list& l, float* norm, int clip, double max_norm, cudaStream_t s) {
+    return l.launches[0].entries.size() <= kSmallTable ? launch_small<NORM, kSmallTable>(l, norm, clip, max_norm, s)
+                                                       : launch_small<NORM, kLargeTable>(l, norm, clip, max_norm, s);
+}
+
+cudaError_t small_by_order(const qrc_list& l, int norm, float* d_norm, int clip, double max_norm, cudaStream_t s) {
+    switch (norm) {
+        case QRC_NORM_1: return run_small<QRC_NORM_1>(l, d_norm, clip, max_norm, s);
+        case QRC_NORM_2: return run_small<QRC_NORM_2>(l, d_norm, clip, max_norm, s);
+        default: return run_small<QRC_NORM_INF>(l, d_norm, clip, max_norm, s);
+    }
+}
+
+template <int NORM>
+cudaError_t run_norm(const qrc_list& l, double* work, float* norm, bool finish, cudaStream_t s) {
     for (const Launch& a : l.launches) {
         const cudaError_t e = a.entries.size() <= kSmallTable ? launch_norm<NORM, kSmallTable>(l, a, work, s)
                                                               : launch_norm<NORM, kLargeTable>(l, a, work, s);
         if (e != cudaSuccess) return e;
     }
+    if (!finish) return cudaSuccess;
     return launch_overlapped(qrc_k_list_finish<NORM>, dim3(1), kThreads, 0, s, 1, work, l.partials, norm);
 }
 
-cudaError_t norm_by_order(const qrc_list& l, int norm, double* work, float* d_norm, cudaStream_t s) {
+cudaError_t norm_by_order(const qrc_list& l, int norm, double* work, float* d_norm, bool finish, cudaStream_t s) {
     switch (norm) {
-        case QRC_NORM_1: return run_norm<QRC_NORM_1>(l, work, d_norm, s);
-        case QRC_NORM_2: return run_norm<QRC_NORM_2>(l, work, d_norm, s);
-        default: return run_norm<QRC_NORM_INF>(l, work, d_norm, s);
+        case QRC_NORM_1: return run_norm<QRC_NORM_1>(l, work, d_norm, finish, s);
+        case QRC_NORM_2: return run_norm<QRC_NORM_2>(l, work, d_norm, finish, s);
+        default: return run_norm<QRC_NORM_INF>(l, work, d_norm, finish, s);
     }
 }
 
@@ -583,29 +706,41 @@ QRC_API int qrc_list_destroy(qrc_list* l) {
     return QRC_OK;
 }
 
-QRC_API size_t qrc_list_workspace(const qrc_list* l) { return l ? (l->partials + 1) * sizeof(double) : 0; }
+QRC_API size_t qrc_list_workspace(const qrc_list* l) {
+    return l && !l->small ? (l->partials + 1) * sizeof(double) : 0;
+}
 
 QRC_API int qrc_list_norm(const qrc_list* l, int norm, float* d_norm, void* d_work, void* stream) {
-    if (!l || !d_norm || !d_work || !known_norm(norm)) return QRC_ERR_INVALID;
-    if (((uintptr_t)d_work & 7) || ((uintptr_t)d_norm & 3)) return QRC_ERR_INVALID;
+    if (!l || !d_norm || !known_norm(norm) || ((uintptr_t)d_norm & 3)) return QRC_ERR_INVALID;
+    if (!l->small && (!d_work || ((uintptr_t)d_work & 7))) return QRC_ERR_INVALID;
     DeviceScope scope(l->device);
     if (!scope.ok) return QRC_ERR_STATE;
-    QRC_CK(norm_by_order(*l, norm, static_cast<double*>(d_work), d_norm, as_stream(stream)));
+    if (l->small) QRC_CK(small_by_order(*l, norm, d_norm, 0, 0.0, as_stream(stream)));
+    else QRC_CK(norm_by_order(*l, norm, static_cast<double*>(d_work), d_norm, true, as_stream(stream)));
     return QRC_OK;
 }
 
 QRC_API int qrc_list_clip(const qrc_list* l, int norm, double max_norm, const float* d_given, float* d_norm,
                           void* d_work, void* stream) {
     if (!l || !known_norm(norm) || !(max_norm >= 0.0) || !l->writable) return QRC_ERR_INVALID;
-    if (!d_given && (!d_work || ((uintptr_t)d_work & 7))) return QRC_ERR_INVALID;
+    if (!d_given && !l->small && (!d_work || ((uintptr_t)d_work & 7))) return QRC_ERR_INVALID;
     if (((uintptr_t)d_given & 3) || ((uintptr_t)d_norm & 3)) return QRC_ERR_INVALID;
     DeviceScope scope(l->device);
     if (!scope.ok) return QRC_ERR_STATE;
     cudaStream_t s = as_stream(stream);
+    if (!d_given && l->small) {
+        QRC_CK(small_by_order(*l, norm, d_norm, 1, max_norm, s));
+        return QRC_OK;
+    }
     double* work = static_cast<double*>(d_work);
-    if (!d_given) QRC_CK(norm_by_order(*l, norm, work, d_norm, s));
-    for (const Launch& a : l->launches)
-        QRC_CK(a.entries.size() <= kSmallTable ? launch_scale<kSmallTable>(*l, a, work, d_given, max_norm, s)
-                                               : launch_scale<kLargeTable>(*l, a, work, d_given, max_norm, s));
+    // Few partial results: the scale pass adds them up, without a launch for it.
+    const bool fold = !d_given && l->launches.size() == 1 && l->partials <= kFold;
+    if (!d_given) QRC_CK(norm_by_order(*l, norm, work, d_norm, !fold, s));
+    for (const Launch& a : l->launches) {
+        const uint32_t count = fold ? l->partials : 0;
+        QRC_CK(a.entries.size() <= kSmallTable
+                   ? launch_scale<kSmallTable>(*l, a, work, d_given, max_norm, norm, count, d_norm, s)
+                   : launch_scale<kLargeTable>(*l, a, work, d_given, max_norm, norm, count, d_norm, s));
+    }
     return QRC_OK;
 }

@@ -19,7 +19,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _native as nat
-from .api import _empty, _stream_handle
+from ._plumbing import empty, stream_handle
 
 _TYPES = {torch.float32: nat.TYPE_F32, torch.bfloat16: nat.TYPE_BF16, torch.float16: nat.TYPE_F16}
 _NORMS = {1.0: nat.NORM_1, 2.0: nat.NORM_2, math.inf: nat.NORM_INF}
@@ -144,7 +144,7 @@ class TensorList:
 
     @staticmethod
     def _order(ord) -> int:
-        code = _NORMS.get(float(ord))
+        code = _NORMS.get(ord)
         if code is None:
             raise RuntimeError(f"TensorList: the norm is of order 1, 2 or inf, got {ord!r}")
         return code
@@ -155,12 +155,17 @@ class TensorList:
         float64; a NaN element gives NaN.  The same bits on every call.
         Asynchronous."""
         code = self._order(ord)
-        out = _empty((), torch.float32, self._torch_device, stream) if out is None else self._scalar(out, "out")
-        work = _empty(self._work_bytes, torch.uint8, self._torch_device, stream)
-        nat.check(self.lib, "qrc_list_norm",
-                  self.lib.qrc_list_norm(self.handle, code, out.data_ptr(), work.data_ptr(),
-                                         _stream_handle(stream, self.device) or None))
+        out = empty((), torch.float32, self._torch_device, stream) if out is None else self._scalar(out, "out")
+        work = self._work(stream)
+        rc = self.lib.qrc_list_norm(self.handle, code, out.data_ptr(), None if work is None else work.data_ptr(),
+                                    stream_handle(stream, self.device))
+        if rc:
+            nat.check(self.lib, "qrc_list_norm", rc)
         return out
+
+    def _work(self, stream):
+        """A workspace for one call; short lists need none."""
+        return empty(self._work_bytes, torch.uint8, self._torch_device, stream) if self._work_bytes else None
 
     def clip_norm(self, max_norm: float, ord: float = 2.0, norm: Optional[torch.Tensor] = None,
                   stream=None) -> torch.Tensor:
@@ -175,14 +180,12 @@ class TensorList:
         if not self._writable:
             raise RuntimeError("TensorList: outputs share memory with one another or with other tensors; "
                                "scaling them would change elements twice")
-        given = 0
         if norm is not None:
             given, result, work = self._scalar(norm, "norm").data_ptr(), norm, None
         else:
-            result = _empty((), torch.float32, self._torch_device, stream)
-            work = _empty(self._work_bytes, torch.uint8, self._torch_device, stream)
-        nat.check(self.lib, "qrc_list_clip",
-                  self.lib.qrc_list_clip(self.handle, code, max_norm, given or None, result.data_ptr(),
-                                         work.data_ptr() if work is not None else None,
-                                         _stream_handle(stream, self.device) or None))
+            given, result, work = None, empty((), torch.float32, self._torch_device, stream), self._work(stream)
+        rc = self.lib.qrc_list_clip(self.handle, code, max_norm, given, result.data_ptr(),
+                                    None if work is None else work.data_ptr(), stream_handle(stream, self.device))
+        if rc:
+            nat.check(self.lib, "qrc_list_clip", rc)
         return result

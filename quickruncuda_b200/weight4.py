@@ -15,7 +15,7 @@ from typing import Optional
 import torch
 
 from . import _native as nat
-from .api import _empty, _stream_handle
+from ._plumbing import empty, stream_handle
 
 _TYPES = {torch.bfloat16: nat.TYPE_BF16, torch.float16: nat.TYPE_F16}
 _OUT_TYPES = {torch.float32: nat.TYPE_F32, **_TYPES}
@@ -79,12 +79,24 @@ class Weight4:
         for name, t in (("packed", packed), ("scales", scales), ("zeros", zeros)):
             if t is not None and not t.is_contiguous():
                 raise RuntimeError(f"Weight4: {name} has to be contiguous")
+        self._set(packed, scales, zeros, n, k, group)
+
+    def _set(self, packed, scales, zeros, n: int, k: int, group: int) -> None:
         self.lib = nat.load()
         self.packed, self.scales, self.zeros = packed, scales, zeros
         self.shape, self.group, self.dtype, self.device = (n, k), group, scales.dtype, packed.device
+        self._index = packed.device.index
         self._w = nat.W4(packed.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(), n, k, group,
                          _TYPES[scales.dtype])
         self._ref = ctypes.byref(self._w)
+
+    @classmethod
+    def _new(cls, n: int, k: int, group: int, dtype, symmetric: bool, device, stream) -> "Weight4":
+        """A matrix with memory of its own, not filled yet."""
+        w4, groups = cls.__new__(cls), (-(-k // group), n)
+        w4._set(empty(packed_shape(n, k), torch.int32, device, stream), empty(groups, dtype, device, stream),
+                None if symmetric else empty(groups, torch.uint8, device, stream), n, k, group)
+        return w4
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
@@ -96,10 +108,9 @@ class Weight4:
             raise RuntimeError(f"Weight4: codes have to be 2-D, got {tuple(codes.shape)}")
         n, k = codes.shape
         ld = _pitch(codes, "codes")
-        w4 = cls(_empty(packed_shape(n, k), torch.int32, codes.device, stream), scales, zeros, k, group)
+        w4 = cls(empty(packed_shape(n, k), torch.int32, codes.device, stream), scales, zeros, k, group)
         nat.check(w4.lib, "qrc_w4_pack",
-                  w4.lib.qrc_w4_pack(codes.device.index, codes.data_ptr(), ld, w4._ref,
-                                     _stream_handle(stream, codes.device.index) or None))
+                  w4.lib.qrc_w4_pack(w4._index, codes.data_ptr(), ld, w4._ref, stream_handle(stream, w4._index)))
         return w4
 
     def dequant(self, out: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None,
@@ -110,12 +121,13 @@ class Weight4:
             dtype = self.dtype if dtype is None else dtype
             if dtype not in _OUT_TYPES:
                 raise RuntimeError(f"Weight4: dequant needs dtype in {tuple(_OUT_TYPES)}, got {dtype}")
-            out = _empty(self.shape, dtype, self.device, stream)
+            out = empty(self.shape, dtype, self.device, stream)
         else:
             _check(out, "out", _OUT_TYPES if dtype is None else (dtype,), self.shape, self.device)
-        nat.check(self.lib, "qrc_w4_dequant",
-                  self.lib.qrc_w4_dequant(self.device.index, self._ref, out.data_ptr(), _pitch(out, "out"),
-                                          _OUT_TYPES[out.dtype], _stream_handle(stream, self.device.index) or None))
+        rc = self.lib.qrc_w4_dequant(self._index, self._ref, out.data_ptr(), _pitch(out, "out"), _OUT_TYPES[out.dtype],
+                                     stream_handle(stream, self._index))
+        if rc:
+            nat.check(self.lib, "qrc_w4_dequant", rc)
         return out
 
     def matvec(self, x: torch.Tensor, bias: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
@@ -124,29 +136,33 @@ class Weight4:
         of that type or, with out_dtype, of float32.  Made for a few rows (a
         decode step).  Sums in float32.  Asynchronous."""
         n, k = self.shape
-        _check(x, "x", (self.dtype,), device=self.device)
-        if x.dim() == 0 or x.shape[-1] != k:
-            raise RuntimeError(f"Weight4: x has shape {tuple(x.shape)}, needs [..., {k}]")
+        if x.dtype is not self.dtype or x.device != self.device:
+            _check(x, "x", (self.dtype,), device=self.device)
+        shape = x.shape
+        if not shape or shape[-1] != k:
+            raise RuntimeError(f"Weight4: x has shape {tuple(shape)}, needs [..., {k}]")
         if bias is not None:
             _check(bias, "bias", (self.dtype,), (n,), self.device)
             if n > 1 and bias.stride(0) != 1:
                 raise RuntimeError("Weight4: bias has to be contiguous")
-        shape = x.shape[:-1] + (n,)
         kind = out_dtype if out_dtype is not None else out.dtype if out is not None else self.dtype
-        if kind != torch.float32 and kind != self.dtype:
+        if kind is not self.dtype and kind is not torch.float32:
             raise RuntimeError(f"Weight4: matvec gives {self.dtype} or float32, got {kind}")
-        if out is None:
-            out = _empty(shape, kind, self.device, stream)
+        if len(shape) == 2:
+            m, x2 = shape[0], x
         else:
-            _check(out, "out", (kind,), shape, self.device)
-        m = x.numel() // k if k else shape[:-1].numel()
-        x2 = _as_rows(x, m, k, "x")
-        y2 = _as_rows(out, m, n, "out")
-        ldx, ldy = _pitch(x2, "x"), _pitch(y2, "out")
-        nat.check(self.lib, "qrc_w4_matvec",
-                  self.lib.qrc_w4_matvec(self.device.index, self._ref, x.data_ptr(), m, ldx,
-                                         None if bias is None else bias.data_ptr(), out.data_ptr(), ldy,
-                                         _OUT_TYPES[kind], _stream_handle(stream, self.device.index) or None))
+            m = shape[:-1].numel()
+            x2 = _as_rows(x, m, k, "x")
+        ldx = k if x.is_contiguous() else _pitch(x2, "x")
+        if out is None:
+            out, ldy = empty((*shape[:-1], n), kind, self.device, stream), n
+        else:
+            _check(out, "out", (kind,), (*shape[:-1], n), self.device)
+            ldy = _pitch(_as_rows(out, m, n, "out"), "out")
+        rc = self.lib.qrc_w4_matvec(self._index, self._ref, x.data_ptr(), m, ldx, None if bias is None else bias.data_ptr(),
+                                    out.data_ptr(), ldy, _OUT_TYPES[kind], stream_handle(stream, self._index))
+        if rc:
+            nat.check(self.lib, "qrc_w4_matvec", rc)
         return out
 
 
@@ -172,10 +188,8 @@ def quant_w4(w: torch.Tensor, group: int = 128, symmetric: bool = True, stream=N
         raise RuntimeError(f"Weight4: w has to be 2-D, got {tuple(w.shape)}")
     n, k = w.shape
     ld = _pitch(w, "w")
-    groups = (-(-k // _check_group(group)), n)
-    w4 = Weight4(_empty(packed_shape(n, k), torch.int32, w.device, stream), _empty(groups, w.dtype, w.device, stream),
-                 None if symmetric else _empty(groups, torch.uint8, w.device, stream), k, group)
-    nat.check(w4.lib, "qrc_w4_quant",
-              w4.lib.qrc_w4_quant(w.device.index, w.data_ptr(), ld, int(bool(symmetric)), w4._ref,
-                                  _stream_handle(stream, w.device.index) or None))
+    w4 = Weight4._new(n, k, _check_group(group), w.dtype, bool(symmetric), w.device, stream)
+    rc = w4.lib.qrc_w4_quant(w4._index, w.data_ptr(), ld, int(bool(symmetric)), w4._ref, stream_handle(stream, w4._index))
+    if rc:
+        nat.check(w4.lib, "qrc_w4_quant", rc)
     return w4
