@@ -38,9 +38,21 @@ template <> struct Half<__nv_bfloat16> {
     using Pair = __nv_bfloat162;
     static constexpr uint32_t kOne = 0x41804180u;
     static constexpr float kBias = 16.0f, kUnit = 1.0f;
-    static constexpr float kMax = 3.3895313892515355e38f;
+    static constexpr float kMax = 3.3895313892515355e38f, kLeastScale = 0x1p-100f, kMostScale = 0x1p100f;
+    // Within four float steps of the middle between two values of the type.
+    static __device__ __forceinline__ bool near_border(float f) { return (__float_as_uint(f) & 0xffffu) - 0x7ffcu <= 8u; }
+    // A pair as two floats.
+    static __device__ __forceinline__ uint64_t widen(uint32_t p) { return (uint64_t)(p & 0xffff0000u) << 32 | p << 16; }
+    // (bits & kCodeMask) | kWide is a constant plus code / kWideUnit, with room
+    // to subtract a zero's and multiply by scale * kWideUnit.
+    static constexpr uint32_t kWide = 0x41804180u;
+    static constexpr float kWideUnit = 1.0f, kLeastWide = kLeastScale;
     static __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
         const Pair r = __hsub2(reinterpret_cast<Pair&>(a), reinterpret_cast<Pair&>(b));
+        return reinterpret_cast<const uint32_t&>(r);
+    }
+    static __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+        const Pair r = __hmul2_rn(reinterpret_cast<Pair&>(a), reinterpret_cast<Pair&>(b));
         return reinterpret_cast<const uint32_t&>(r);
     }
     static __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -56,9 +68,20 @@ template <> struct Half<__half> {
     using Pair = __half2;
     static constexpr uint32_t kOne = 0u;
     static constexpr float kBias = 0.0f, kUnit = 0x1p-21f;
-    static constexpr float kMax = 65504.0f;
+    static constexpr float kMax = 65504.0f, kLeastScale = 0x1p-13f, kMostScale = 65504.0f;
+    static __device__ __forceinline__ bool near_border(float f) { return (__float_as_uint(f) & 0x1fffu) - 0x0ffcu <= 8u; }
+    static __device__ __forceinline__ uint64_t widen(uint32_t p) {
+        const float2 f = __half22float2(reinterpret_cast<__half2&>(p));
+        return (uint64_t)__float_as_uint(f.y) << 32 | __float_as_uint(f.x);
+    }
+    static constexpr uint32_t kWide = 0x64006400u;
+    static constexpr float kWideUnit = 0.125f, kLeastWide = 0x1p-11f;     // an eighth is exact
     static __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
         const Pair r = __hsub2(reinterpret_cast<Pair&>(a), reinterpret_cast<Pair&>(b));
+        return reinterpret_cast<const uint32_t&>(r);
+    }
+    static __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+        const Pair r = __hmul2_rn(reinterpret_cast<Pair&>(a), reinterpret_cast<Pair&>(b));
         return reinterpret_cast<const uint32_t&>(r);
     }
     static __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
@@ -75,6 +98,8 @@ template <class T> __device__ __forceinline__ T from_bits(uint32_t b) {
     const uint16_t h = (uint16_t)b;
     return reinterpret_cast<const T&>(h);
 }
+
+template <class T> __device__ __forceinline__ uint32_t to_bits(T x) { return reinterpret_cast<const uint16_t&>(x); }
 
 __device__ __forceinline__ uint32_t rotate_right(uint32_t w, int by) { return __funnelshift_r(w, w, by); }
 
@@ -98,6 +123,13 @@ __device__ __forceinline__ uint64_t word_at(uint64_t row, uint64_t tile, uint64_
     return ((row >> 4) * tiles + tile) * 256 + (row & 15) * 16 + i;
 }
 
+// Blocks of four warps, a warp per 4 or 8 rows and 256 columns.  A 16384 x 8192
+// matrix of bf16 quantizes in 70 us with eight rows loaded at a time, 77 with
+// four; with zeros (more registers) or unaligned rows (more instructions per
+// load) it is the other way round: fp16 with zeros 114 and 105 us.
+constexpr int kWindowWarps = 4, kWindowThreads = 32 * kWindowWarps, kDequantRows = 8;
+template <bool SYMMETRIC, bool VEC> constexpr int kQuantRows = SYMMETRIC && VEC ? 8 : 4;
+
 // -- quantize --------------------------------------------------------------------
 
 // The largest and smallest of a group leave out infinities and NaN.
@@ -117,58 +149,257 @@ template <class T> __device__ __forceinline__ float round_once(double d) {
            : Half<T>::to_float(Half<T>::round(nudged));
 }
 
-// One warp takes 256 columns of a row at a time, eight columns per lane, so a
-// group is 4 to 32 neighbouring lanes.
+// Eight neighbouring 16-bit elements at p, of which those from `have` on are
+// 0.  `lo` and `hi` bound the memory of the whole matrix.  A row that does not
+// start on 16 bytes is read as two aligned vectors, shifted together.
+template <bool VEC>
+__device__ __forceinline__ uint4 load_eight(const uint16_t* p, int have, const uint16_t* lo, const uint16_t* hi) {
+    if (VEC && have >= 8) return *reinterpret_cast<const uint4*>(p);
+    const uint32_t off = (uint32_t)(uintptr_t)p & 15;
+    const uint16_t* const base = p - off / 2;
+    if (!VEC && have >= 8 && base >= lo && base + 16 <= hi) {
+        const uint4 u = *reinterpret_cast<const uint4*>(base), v = *(reinterpret_cast<const uint4*>(base) + 1);
+        uint32_t w[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+        if (off & 8) {
+#pragma unroll
+            for (int i = 0; i < 6; i++) w[i] = w[i + 2];
+        }
+        if (off & 4) {
+#pragma unroll
+            for (int i = 0; i < 5; i++) w[i] = w[i + 1];
+        }
+        const uint32_t bits = (off & 2) * 8;
+        return make_uint4(__funnelshift_r(w[0], w[1], bits), __funnelshift_r(w[1], w[2], bits),
+                          __funnelshift_r(w[2], w[3], bits), __funnelshift_r(w[3], w[4], bits));
+    }
+    uint32_t e[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) e[i] = i < have ? p[i] : 0u;
+    return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+}
+
+// One row's eight columns of a lane, any values: scale, zero and codes from
+// the definition.  `lanes` neighbouring lanes share a group.
 template <class T>
-__global__ void __launch_bounds__(256)
-qrc_k_w4_quant(const T* w, uint64_t ld, uint64_t n, uint64_t k, int group, int symmetric, int vec,
-               uint32_t* packed, T* scales, uint8_t* zeros) {
+__device__ __noinline__ uint32_t quant_any(uint4 v, int lanes, bool symmetric, float* scale, float* zero) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    float x[8], most = 0.0f, least = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        x[i] = Half<T>::to_float(from_bits<T>(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu));
+        const float f = finite_or_zero(x[i]);
+        most = fmaxf(most, symmetric ? fabsf(f) : f);
+        least = fminf(least, f);
+    }
+    for (int d = lanes / 2; d; d >>= 1) {
+        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+        least = fminf(least, __shfl_xor_sync(0xffffffffu, least, d));
+    }
+    const float s = symmetric ? Half<T>::to_float(Half<T>::round(__fdiv_rn(most, 7.0f)))
+                              : round_once<T>(((double)most - (double)least) / 15.0);
+    // Quotients of two 16-bit floats keep their side of every border i + 1/2
+    // in 32 bits: they are on it or 2^-16 away at least.
+    float z = symmetric ? 8.0f : 0.0f;
+    if (!symmetric && s > 0.0f) z = fminf(fmaxf(rintf(__fdiv_rn(-least, s)), 0.0f), 15.0f);
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        float c = z;
+        if (s > 0.0f && x[i] == x[i]) c = fminf(fmaxf(rintf(__fdiv_rn(x[i], s)) + z, symmetric ? 1.0f : 0.0f), 15.0f);
+        word |= place_code((uint32_t)c, i);
+    }
+    *scale = s;
+    *zero = z;
+    return word;
+}
+
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// A reciprocal good to about one step; what is divided with it is corrected.
+__device__ __forceinline__ float reciprocal(float x) {
+    float r;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// x / s for pairs, s given as its reciprocal r and -s: a product, the
+// remainder it leaves and its correction.  The remainder is exact up to one
+// rounding, so a quotient that float can hold (every whole number and every
+// border i + 1/2) comes out exactly.
+__device__ __forceinline__ uint64_t divide2(uint64_t x, uint64_t r, uint64_t minus_s) {
+    const uint64_t p = mul2(x, r);
+    return fma2(fma2(p, minus_s, x), r, p);
+}
+
+// One warp takes ROWS rows by 256 columns, eight columns per lane and row, so a
+// group is LANES = 4 to 32 neighbouring lanes.  Bound by instructions as much as by memory: magnitudes are compared
+// as pairs of 16 bits, two rows (or maximum and minimum) per shuffle, and
+// quotients are formed in pairs without a division.  Rows with infinities,
+// NaN or scales near the ends of the type's range go through quant_any.
+template <class T, bool SYMMETRIC, int LANES, bool VEC>
+__global__ void __launch_bounds__(kWindowThreads)
+qrc_k_w4_quant(const uint16_t* w, uint64_t ld, uint64_t n, uint64_t k, uint32_t* packed, uint16_t* scales, uint8_t* zeros) {
     qrc::griddep_wait();
     qrc::griddep_launch_dependents();
-    const int lane = threadIdx.x & 31;
-    const uint64_t tiles = (k + 127) / 128, windows = (k + 255) / 256;
-    const uint64_t tasks = (n + 15) / 16 * 16 * windows;
-    for (uint64_t task = (uint64_t)blockIdx.x * 8 + (threadIdx.x >> 5); task < tasks; task += (uint64_t)gridDim.x * 8) {
-        const uint64_t row = task / windows, k0 = (task - row * windows) * 256 + lane * 8;
-        const T* p = w + row * ld + k0;
-        T v[8];
-        if (vec && row < n && k0 + 8 <= k) *reinterpret_cast<uint4*>(v) = *reinterpret_cast<const uint4*>(p);
-        else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = row < n && k0 + i < k ? p[i] : Half<T>::round(0.0f);
-        }
-        float x[8], most = 0.0f, least = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            x[i] = Half<T>::to_float(v[i]);
-            const float f = finite_or_zero(x[i]);
-            most = fmaxf(most, symmetric ? fabsf(f) : f);
-            least = fminf(least, f);
-        }
-        for (int d = group / 16; d; d >>= 1) {
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-            least = fminf(least, __shfl_xor_sync(0xffffffffu, least, d));
-        }
-        const float s = symmetric ? Half<T>::to_float(Half<T>::round(__fdiv_rn(most, 7.0f)))
-                                  : round_once<T>(((double)most - (double)least) / 15.0);
-        // Quotients of two 16-bit floats keep their side of every border
-        // i + 1/2 in 32 bits: they are on it or 2^-16 away at least.
-        float z = symmetric ? 8.0f : 0.0f;
-        if (!symmetric && s > 0.0f) z = fminf(fmaxf(rintf(__fdiv_rn(-least, s)), 0.0f), 15.0f);
-        const float low = symmetric ? 1.0f : 0.0f;
-        uint32_t word = 0;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            float c = z;
-            if (s > 0.0f && x[i] == x[i]) c = fminf(fmaxf(rintf(__fdiv_rn(x[i], s)) + z, low), 15.0f);
-            word |= place_code((uint32_t)c, i);
-        }
+    using Pair = typename Half<T>::Pair;
+    constexpr int ROWS = kQuantRows<SYMMETRIC, VEC>;
+    const int lane = threadIdx.x & 31, member = lane % LANES;
+    const uint64_t tiles = (k + 127) / 128, windows = (k + 255) / 256, tasks = (n + 15) / 16 * (16 / ROWS) * windows;
+    const uint16_t* const end = w + (n - 1) * ld + k;
+    for (uint64_t task = (uint64_t)blockIdx.x * kWindowWarps + (threadIdx.x >> 5); task < tasks; task += (uint64_t)gridDim.x * kWindowWarps) {
+        const uint64_t part = task / windows, first = part * ROWS, k0 = (task - part * windows) * 256 + lane * 8;
+        const int have = k0 < k ? (int)min((uint64_t)8, k - k0) : 0;
         const uint64_t tile = k0 >> 7;
-        const uint32_t i16 = lane & 15;
-        if (tile < tiles) packed[word_at(row, tile, tiles, (i16 & 3) * 4 + (i16 >> 2))] = word;
-        if (k0 % group == 0 && k0 < k && row < n) {
-            scales[k0 / group * n + row] = Half<T>::round(s);
-            if (!symmetric) zeros[k0 / group * n + row] = (uint8_t)z;
+        uint32_t* const to = packed + ((first >> 4) * tiles + tile) * 256 + (first & 15) * 16 + (lane & 3) * 4 + ((lane >> 2) & 3);
+        uint4 v[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) {
+            const uint64_t row = first + r;
+            v[r] = row < n && have ? load_eight<VEC>(w + row * ld + k0, have, w, end) : make_uint4(0, 0, 0, 0);
+        }
+        auto as_pair = [](uint32_t x) { return reinterpret_cast<Pair&>(x); };
+        auto as_bits = [](Pair x) { return reinterpret_cast<uint32_t&>(x); };
+        // SYMMETRIC: the largest magnitudes of rows 2*i and 2*i + 1.
+        // Otherwise a row's maximum and negated minimum, 0 included.
+        uint32_t most[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) {
+            const Pair a = as_pair(v[r].x), b = as_pair(v[r].y), c = as_pair(v[r].z), d = as_pair(v[r].w);
+            if (SYMMETRIC) most[r] = as_bits(__hmax2_nan(__hmax2_nan(__habs2(a), __habs2(b)), __hmax2_nan(__habs2(c), __habs2(d))));
+            else {
+                const uint32_t up = as_bits(__hmax2_nan(__hmax2_nan(a, b), __hmax2_nan(c, d)));
+                const uint32_t down = as_bits(__hmin2_nan(__hmin2_nan(a, b), __hmin2_nan(c, d))) ^ 0x80008000u;
+                most[r] = as_bits(__hmax2_nan(__hmax2_nan(as_pair(__byte_perm(up, down, 0x5410)), as_pair(__byte_perm(up, down, 0x7632))),
+                                              as_pair(0u)));
+            }
+        }
+        if (SYMMETRIC) {
+#pragma unroll
+            for (int r = 0; r < ROWS; r += 2)
+                most[r / 2] = as_bits(__hmax2_nan(as_pair(__byte_perm(most[r], most[r + 1], 0x5410)),
+                                                  as_pair(__byte_perm(most[r], most[r + 1], 0x7632))));
+        }
+        constexpr int COUNT = SYMMETRIC ? ROWS / 2 : ROWS;
+        bool usual = true;
+        uint32_t scale[ROWS];
+        float s[ROWS], zero[ROWS];
+#pragma unroll
+        for (int i = 0; i < COUNT; i++) {
+#pragma unroll
+            for (int d = LANES / 2; d; d >>= 1)
+                most[i] = as_bits(__hmax2_nan(as_pair(most[i]), as_pair(__shfl_xor_sync(0xffffffffu, most[i], d))));
+            const float first = Half<T>::to_float(from_bits<T>(most[i] & 0xffffu)), second = Half<T>::to_float(from_bits<T>(most[i] >> 16));
+            if (SYMMETRIC) {
+                // A seventh of a 16-bit float is 2^-15 of itself away from
+                // every border of the type: a product rounds as the quotient.
+                const T a = Half<T>::round(first * (1.0f / 7.0f)), b = Half<T>::round(second * (1.0f / 7.0f));
+                s[2 * i] = Half<T>::to_float(a);
+                s[2 * i + 1] = Half<T>::to_float(b);
+                scale[2 * i] = to_bits(a);
+                scale[2 * i + 1] = to_bits(b);
+                zero[2 * i] = zero[2 * i + 1] = 8.0f;
+            } else {
+                // The difference, exact as sum and error; its fifteenth in
+                // float decides unless it is within four steps of a border.
+                const float sum = first + second, t = sum - first, miss = (first - (sum - t)) + (second - t);
+                const float f = sum * (1.0f / 15.0f);
+                T a = Half<T>::round(f);
+                if (Half<T>::near_border(f)) {
+                    const float exact = round_once<T>(((double)sum + (double)miss) / 15.0);
+                    a = Half<T>::round(exact);
+                }
+                s[i] = Half<T>::to_float(a);
+                scale[i] = to_bits(a);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) usual = usual && (s[r] == 0.0f || (s[r] >= Half<T>::kLeastScale && s[r] <= Half<T>::kMostScale));
+        if (__any_sync(0xffffffffu, !usual)) {
+#pragma unroll 1
+            for (int r = 0; r < ROWS; r++) {
+                const uint64_t row = first + r;
+                const uint4 x = row < n && have ? load_eight<VEC>(w + row * ld + k0, have, w, end) : make_uint4(0, 0, 0, 0);
+                float sr, zr;
+                const uint32_t word = quant_any<T>(x, LANES, SYMMETRIC, &sr, &zr);
+                if (tile < tiles) to[r * 16] = word;
+                if (member == 0 && have && row < n) {
+                    const uint64_t at = k0 / (LANES * 8) * n + row;
+                    scales[at] = (uint16_t)to_bits(Half<T>::round(sr));
+                    if (!SYMMETRIC) zeros[at] = (uint8_t)zr;
+                }
+            }
+            continue;
+        }
+#pragma unroll
+        for (int r = 0; r < ROWS; r++) {
+            const float inv = s[r] > 0.0f ? reciprocal(s[r]) : 0.0f;
+            const uint64_t r2 = pair_of(inv, inv), minus_s = pair_of(-s[r], -s[r]);
+            constexpr float kRound = 12582912.0f;               // 1.5 * 2^23: adding it rounds to whole numbers
+            if (!SYMMETRIC) {
+                const float least = Half<T>::to_float(from_bits<T>(most[r] >> 16));      // -minimum
+                float z0, z1;
+                const uint64_t q = add2(divide2(pair_of(least, 0.0f), r2, minus_s), pair_of(kRound, kRound));
+                asm("mov.b64 {%0, %1}, %2;" : "=f"(z0), "=f"(z1) : "l"(q));
+                zero[r] = z0 - kRound;
+            }
+            const uint32_t x[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
+            uint32_t p[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                uint64_t q = divide2(Half<T>::widen(x[i]), r2, minus_s);
+                uint32_t c0, c1;
+                if (SYMMETRIC) {
+                    q = add2(q, pair_of(kRound + 8.0f, kRound + 8.0f));
+                    asm("mov.b64 {%0, %1}, %2;" : "=r"(c0), "=r"(c1) : "l"(q));
+                } else {
+                    float f0, f1;
+                    q = add2(add2(q, pair_of(kRound, kRound)), pair_of(zero[r], zero[r]));
+                    asm("mov.b64 {%0, %1}, %2;" : "=f"(f0), "=f"(f1) : "l"(q));
+                    c0 = __float_as_uint(fminf(f0, kRound + 15.0f));
+                    c1 = __float_as_uint(fminf(f1, kRound + 15.0f));
+                }
+                p[i] = __byte_perm(c0, c1, 0x5410);             // the codes are the last bits
+            }
+            const uint32_t word = p[0] + p[1] * 16u + p[2] * 256u + p[3] * 4096u;
+            if (tile < tiles) to[r * 16] = __funnelshift_l(word, word, 3);
+        }
+        // Scales: row i by the group's lane i, LANES rows at a time, for
+        // groups that start in front of column k.
+        if (k0 - member * 8 < k) {
+#pragma unroll
+            for (int r0 = 0; r0 < ROWS; r0 += LANES) {
+                uint32_t mine = 0;
+                float z = 0.0f;
+#pragma unroll
+                for (int r = r0; r < r0 + LANES && r < ROWS; r++) {
+                    if (member == r - r0) { mine = scale[r]; z = zero[r]; }
+                }
+                const uint64_t row = first + r0 + member;
+                if (member < ROWS - r0 && row < n) {
+                    const uint64_t at = k0 / (LANES * 8) * n + row;
+                    scales[at] = (uint16_t)mine;
+                    if (!SYMMETRIC) zeros[at] = (uint8_t)z;
+                }
+            }
         }
     }
 }
@@ -206,31 +437,127 @@ template <> __device__ __forceinline__ __half round_to<__half>(float x) {
     return Half<__half>::round(x > m ? m : x < -m ? -m : x);
 }
 
-template <class T, class TO>
-__global__ void __launch_bounds__(256)
-qrc_k_w4_dequant(const uint32_t* packed, const T* scales, const uint8_t* zeros, uint64_t n, uint64_t k, int group,
-                 TO* out, uint64_t ld, int vec) {
+// Writes a lane's eight values of a row, `v` as 16 * WORDS bytes, of which
+// `have` elements are in front of the last column.  VEC: the row starts on 16
+// bytes.  Otherwise the lanes trade what is off by, so that whole aligned
+// vectors are written inside a window of 32 lanes, and single elements at its
+// ends.
+template <class TO, bool VEC>
+__device__ __forceinline__ void store_eight(TO* p, const uint32_t (&v)[2 * sizeof(TO)], int have, int lane, bool row_ok) {
+    constexpr int WORDS = 2 * sizeof(TO), E = 4 / sizeof(TO);       // 32-bit words of eight, elements of a word
+    if (VEC) {
+        if (!row_ok || have <= 0) return;
+        if (have >= 8) {
+#pragma unroll
+            for (int i = 0; i < WORDS / 4; i++)
+                reinterpret_cast<uint4*>(p)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            return;
+        }
+    } else {
+        // Word i of the lane below, then the own ones: the aligned vectors
+        // that end within this lane's columns start `off` bytes before it.
+        const uint32_t off = (uint32_t)(uintptr_t)p & 15;
+        uint32_t w[WORDS + 4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = __shfl_up_sync(0xffffffffu, v[WORDS - 4 + i], 1);
+#pragma unroll
+        for (int i = 0; i < WORDS; i++) w[4 + i] = v[i];
+        const bool below = lane > 0;
+        const bool next_whole = __shfl_down_sync(0xffffffffu, (int)(have >= 8), 1) && lane < 31;
+        if (!row_ok || have <= 0) return;
+        if (off != 0 && have >= 8) {
+            // shift the words up so that w[4 ..] starts at the aligned address p - off
+            uint32_t u[WORDS + 4];
+#pragma unroll
+            for (int i = 0; i < WORDS + 4; i++) u[i] = w[i];
+            if (off & 8) {
+#pragma unroll
+                for (int i = WORDS + 3; i >= 2; i--) u[i] = u[i - 2];
+            }
+            if (off & 4) {
+#pragma unroll
+                for (int i = WORDS + 3; i >= 1; i--) u[i] = u[i - 1];
+            }
+            const uint32_t bits = (off & 2) * 8;
+            uint32_t o[WORDS];
+#pragma unroll
+            for (int i = 0; i < WORDS; i++) o[i] = __funnelshift_l(u[3 + i], u[4 + i], bits);
+            uint4* const at = reinterpret_cast<uint4*>(reinterpret_cast<char*>(p) - off);
+#pragma unroll
+            for (int i = 0; i < WORDS / 4; i++)
+                if (i > 0 || below) at[i] = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+            // the window's first vector starts before it, its last one ends behind it
+            const int head = below ? 0 : (16 - (int)off) / (int)sizeof(TO), tail = next_whole ? 8 : 8 - (int)off / (int)sizeof(TO);
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (e < head || e >= tail) {
+                    const uint32_t word = v[e / E];
+                    if (sizeof(TO) == 4) reinterpret_cast<uint32_t*>(p)[e] = word;
+                    else reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(word >> (e % E * 16));
+                }
+            return;
+        }
+        if (have >= 8) {
+#pragma unroll
+            for (int i = 0; i < WORDS / 4; i++)
+                reinterpret_cast<uint4*>(p)[i] = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+            return;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        if (e < have) {
+            const uint32_t word = v[e / E];
+            if (sizeof(TO) == 4) reinterpret_cast<uint32_t*>(p)[e] = word;
+            else reinterpret_cast<uint16_t*>(p)[e] = (uint16_t)(word >> (e % E * 16));
+        }
+}
+
+// One warp takes ROWS rows by 256 columns, eight columns per lane and row.  Into
+// the scales' own type the differences code - zero, exact in 16 bits, are
+// multiplied by the scale in pairs, which rounds once; scales near the ends of
+// the type's range, and other types, go through float.
+template <class T, class TO, bool VEC>
+__global__ void __launch_bounds__(kWindowThreads)
+qrc_k_w4_dequant(const uint32_t* packed, const uint16_t* scales, const uint8_t* zeros, uint64_t n, uint64_t k,
+                 int group_log2, TO* out, uint64_t ld) {
     qrc::griddep_wait();
     qrc::griddep_launch_dependents();
-    const uint64_t tiles = (k + 127) / 128, total = (n + 15) / 16 * tiles * 256;
-    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) {
-        const uint64_t tile = i >> 8, above = tile / tiles;
-        const uint64_t row = above * 16 + ((i >> 4) & 15), col = (tile - above * tiles) * 128 + word_column(i & 15);
-        if (row >= n || col >= k) continue;
-        const uint32_t word = packed[i];
-        const uint64_t at = col / group * n + row;
-        const float s = Half<T>::to_float(scales[at]);
-        const float z = zeros ? (float)zeros[at] : 8.0f;
-        __align__(16) TO v[8];
+    constexpr int ROWS = kDequantRows, WORDS = 2 * sizeof(TO);
+    const int lane = threadIdx.x & 31;
+    const uint64_t tiles = (k + 127) / 128, windows = (k + 255) / 256, tasks = (n + 15) / 16 * (16 / ROWS) * windows;
+    for (uint64_t task = (uint64_t)blockIdx.x * kWindowWarps + (threadIdx.x >> 5); task < tasks; task += (uint64_t)gridDim.x * kWindowWarps) {
+        const uint64_t part = task / windows, first = part * ROWS, k0 = (task - part * windows) * 256 + lane * 8;
+        const int have = k0 < k ? (int)min((uint64_t)8, k - k0) : 0;
+        const uint32_t* const from = packed + ((first >> 4) * tiles + (k0 >> 7)) * 256 + (first & 15) * 16 + (lane & 3) * 4 + ((lane >> 2) & 3);
+        uint32_t word[ROWS], scale[ROWS], zero[ROWS];
+        const uint64_t at = (k0 >> group_log2) * n + first;
 #pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = round_to<TO>(((float)(rotate_right(word, code_shift(e)) & 15u) - z) * s);
-        TO* q = out + row * ld + col;
-        if (vec && col + 8 <= k) {
+        for (int r = 0; r < ROWS; r++) {
+            const bool there = have && first + r < n;
+            word[r] = there ? __ldg(from + r * 16) : 0;
+            scale[r] = there ? __ldg(scales + at + r) : 0;
+            zero[r] = there && zeros ? __ldg(zeros + at + r) : 8;
+        }
 #pragma unroll
-            for (int e = 0; e < (int)sizeof(v) / 16; e++) reinterpret_cast<uint4*>(q)[e] = reinterpret_cast<uint4*>(v)[e];
-        } else {
+        for (int r = 0; r < ROWS; r++) {
+            uint32_t v[WORDS];
+            const float s = Half<T>::to_float(from_bits<T>(scale[r]));
+            if (std::is_same<T, TO>::value && s >= Half<T>::kLeastWide && s <= Half<T>::kMax / 16) {
+                const uint32_t m = to_bits(Half<T>::round(s * Half<T>::kWideUnit)) * 0x10001u;
+                const uint32_t z = zero[r] * 0x80008u | Half<T>::kWide;
 #pragma unroll
-            for (int e = 0; e < 8; e++) if (col + e < k) q[e] = v[e];
+                for (int i = 0; i < 4; i++)
+                    v[i] = Half<T>::mul2(Half<T>::sub2((rotate_right(word[r], 4 * i) & kCodeMask) | Half<T>::kWide, z), m);
+            } else {
+                __align__(16) TO f[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    f[e] = round_to<TO>(((float)(rotate_right(word[r], code_shift(e)) & 15u) - (float)zero[r]) * s);
+#pragma unroll
+                for (int i = 0; i < WORDS; i++) v[i] = reinterpret_cast<const uint32_t*>(f)[i];
+            }
+            store_eight<TO, VEC>(out + (first + r) * ld + k0, v, have, lane, first + r < n);
         }
     }
 }
@@ -731,7 +1058,7 @@ inline bool touches(const qrc_w4& w, const void* p, uint64_t bytes) {
 }
 
 dim3 grid_for(uint64_t items, uint64_t per_block) {
-    return dim3((unsigned)std::min<uint64_t>((items + per_block - 1) / per_block, 1u << 16));
+    return dim3((unsigned)std::min<uint64_t>((items + per_block - 1) / per_block, 1u << 20));
 }
 
 // Shared memory a block may have, and what its static part takes.
@@ -781,30 +1108,51 @@ int launch_matvec(const qrc_w4& w, const void* d_x, uint64_t m, uint64_t ldx, co
     return QRC_OK;
 }
 
+// A warp per `rows` rows and 256 columns.
+dim3 grid_for_windows(const qrc_w4& w, int rows) { return grid_for((w.n + 15) / 16 * (16 / rows) * ((w.k + 255) / 256), kWindowWarps); }
+
+template <class T, class TO>
+cudaError_t launch_dequant_to(const qrc_w4& w, TO* out, uint64_t ld, cudaStream_t s) {
+    auto go = [&](auto kernel) {
+        return launch_overlapped(kernel, grid_for_windows(w, kDequantRows), kWindowThreads, 0, s, 1, (const uint32_t*)w.d_packed,
+                                 static_cast<const uint16_t*>(w.d_scales), (const uint8_t*)w.d_zeros, w.n, w.k,
+                                 log2_of(w.group), out, ld);
+    };
+    return rows_aligned(out, ld, w.n, sizeof(TO)) ? go(qrc_k_w4_dequant<T, TO, true>) : go(qrc_k_w4_dequant<T, TO, false>);
+}
+
 template <class T>
 cudaError_t launch_dequant(const qrc_w4& w, void* out, uint64_t ld, int type, cudaStream_t s) {
-    const uint64_t words = qrc_w4_words(w.n, w.k);
-    const int vec = rows_aligned(out, ld, w.n, type == QRC_F32 ? 4 : 2);
-    const T* scales = static_cast<const T*>(w.d_scales);
-    auto go = [&](auto* to) {
-        using TO = std::remove_pointer_t<decltype(to)>;
-        return launch_overlapped(qrc_k_w4_dequant<T, TO>, grid_for(words, 256), 256, 0, s, 1,
-                                 (const uint32_t*)w.d_packed, scales, (const uint8_t*)w.d_zeros, w.n, w.k, w.group, to,
-                                 ld, vec);
-    };
     switch (type) {
-        case QRC_F32: return go(static_cast<float*>(out));
-        case QRC_BF16: return go(static_cast<__nv_bfloat16*>(out));
-        default: return go(static_cast<__half*>(out));
+        case QRC_F32: return launch_dequant_to<T>(w, static_cast<float*>(out), ld, s);
+        case QRC_BF16: return launch_dequant_to<T>(w, static_cast<__nv_bfloat16*>(out), ld, s);
+        default: return launch_dequant_to<T>(w, static_cast<__half*>(out), ld, s);
+    }
+}
+
+template <class T, bool SYMMETRIC, int LANES>
+cudaError_t launch_quant_group(const qrc_w4& w, const void* d_w, uint64_t ld, cudaStream_t s) {
+    auto go = [&](auto kernel, int rows) {
+        return launch_overlapped(kernel, grid_for_windows(w, rows), kWindowThreads, 0, s, 1, static_cast<const uint16_t*>(d_w), ld, w.n,
+                                 w.k, w.d_packed, static_cast<uint16_t*>(w.d_scales), w.d_zeros);
+    };
+    return rows_aligned(d_w, ld, w.n, 2) ? go(qrc_k_w4_quant<T, SYMMETRIC, LANES, true>, kQuantRows<SYMMETRIC, true>)
+                                         : go(qrc_k_w4_quant<T, SYMMETRIC, LANES, false>, kQuantRows<SYMMETRIC, false>);
+}
+
+template <class T, bool SYMMETRIC>
+cudaError_t launch_quant_kind(const qrc_w4& w, const void* d_w, uint64_t ld, cudaStream_t s) {
+    switch (w.group) {
+        case 32: return launch_quant_group<T, SYMMETRIC, 4>(w, d_w, ld, s);
+        case 64: return launch_quant_group<T, SYMMETRIC, 8>(w, d_w, ld, s);
+        case 128: return launch_quant_group<T, SYMMETRIC, 16>(w, d_w, ld, s);
+        default: return launch_quant_group<T, SYMMETRIC, 32>(w, d_w, ld, s);
     }
 }
 
 template <class T>
 cudaError_t launch_quant(const qrc_w4& w, const void* d_w, uint64_t ld, int symmetric, cudaStream_t s) {
-    const int vec = rows_aligned(d_w, ld, w.n, 2);
-    return launch_overlapped(qrc_k_w4_quant<T>, grid_for((w.n + 15) / 16 * 16 * ((w.k + 255) / 256), 8), 256, 0, s, 1,
-                             static_cast<const T*>(d_w), ld, w.n, w.k, w.group, symmetric, vec, w.d_packed,
-                             static_cast<T*>(w.d_scales), w.d_zeros);
+    return symmetric ? launch_quant_kind<T, true>(w, d_w, ld, s) : launch_quant_kind<T, false>(w, d_w, ld, s);
 }
 
 }  // namespace
