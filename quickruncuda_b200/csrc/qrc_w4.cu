@@ -589,26 +589,33 @@ template <int PAIRS> __device__ __forceinline__ void add_scaled(float& c0, float
         : "+f"(c0), "+f"(c1) : "f"(a), "f"(b0), "f"(b1));
 }
 
+// Sixteen bytes of shared memory at a 32-bit address: cheaper to compute than a pointer.
+__device__ __forceinline__ uint4 load_shared(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+
 __device__ __forceinline__ void mma_bytes(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Shape of a block: W warps that each work on R rows of tiles, with NT * 8
+// Shape of a block: W warps that each work on a row of tiles, with NT * 8
 // columns of the matrix instruction and D slots of BT tile columns in flight.
 // DIGITS: the activations as whole numbers, three columns each; see below.
-template <bool DIGITS_, int NT_, int W_, int R_, int BT_, int D_>
+template <bool DIGITS_, int NT_, int W_, int BT_, int D_>
 struct Shape {
     static constexpr bool DIGITS = DIGITS_;
-    static constexpr int NT = NT_, W = W_, R = R_, BT = BT_, D = D_;
+    static constexpr int NT = NT_, W = W_, BT = BT_, D = D_;
     static constexpr int kTokens = DIGITS ? 8 * NT / 3 : 8 * NT;        // rows of activations at a time
     static constexpr int kColumns = DIGITS ? 3 : 1;                     // matrix columns of one of them
     static constexpr int kRowBytes = DIGITS ? 128 : 256;                // of a column, per tile
-    static constexpr int kSlot = BT * R * 1024;                         // bytes
+    static constexpr int kSlot = BT * 1024;                             // bytes
     static constexpr int kRing = W * D * kSlot, kBars = W * D * 8 + 16;
     static constexpr int kBuffers = DIGITS ? 1 : 2;                     // chunks of activations held
-    static_assert(16 * R * 8 * NT * 4 <= D * kSlot, "a warp's sums have to fit in its slots");
+    static_assert(16 * 8 * NT * 4 <= D * kSlot, "a warp's sums have to fit in its slots");
     // Shared memory a tile column of activations takes, and what does not
     // depend on their number.
     static constexpr uint64_t per_tile(uint64_t tokens, int sub) {
@@ -646,7 +653,7 @@ __global__ void __launch_bounds__(S::W * 32, 1)
 qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias, void* y, uint64_t ldy, int y_float,
                 int x_vec, uint32_t chunk_tiles) {
     constexpr bool DIGITS = S::DIGITS;
-    constexpr int NT = S::NT, W = S::W, R = S::R, BT = S::BT, D = S::D, kPer = (SUB + 1) / 2;
+    constexpr int NT = S::NT, W = S::W, BT = S::BT, D = S::D, kUnits = BT * SUB / 2;
     using Sum = std::conditional_t<DIGITS, int, float>;
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ int s_failed;
@@ -656,7 +663,7 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias,
     const uint32_t tiles = (uint32_t)((w.k + 127) / 128);
     const uint32_t groups = (uint32_t)((w.k + (1ull << w.group_log2) - 1) >> w.group_log2);
     const uint32_t chunks = (tiles + chunk_tiles - 1) / chunk_tiles;
-    const uint64_t row_tiles = (w.n + 15) / 16, units = (row_tiles + R - 1) / R;
+    const uint64_t row_tiles = (w.n + 15) / 16;
     const uint32_t pitch = chunk_tiles * S::kRowBytes + 64;     // columns of activations, apart in the banks
     unsigned char* const ring = smem + warp * (D * S::kSlot);
     const uint32_t smem_at = (uint32_t)__cvta_generic_to_shared(smem);
@@ -681,13 +688,12 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias,
     qrc::griddep_launch_dependents();
 
     // Eight activations from column k0 on, zero behind the last column.
+    const uint16_t* const x_bits = reinterpret_cast<const uint16_t*>(x);
+    const uint16_t* const x_end = x_bits + (m - 1) * ldx + w.k;
     auto load_x = [&](int tok, uint64_t k0) {
-        const T* p = x + (m0 + tok) * ldx + k0;
-        if (x_vec && k0 + 8 <= w.k) return *reinterpret_cast<const uint4*>(p);
-        uint32_t e[8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) e[j] = k0 + j < w.k ? reinterpret_cast<const uint16_t*>(p)[j] : 0u;
-        return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+        const uint16_t* p = x_bits + (m0 + tok) * ldx + k0;
+        const int have = k0 < w.k ? (int)min((uint64_t)8, w.k - k0) : 0;
+        return x_vec ? load_eight<true>(p, have, x_bits, x_end) : load_eight<false>(p, have, x_bits, x_end);
     };
     // Brings a chunk's activations to shared memory, zero behind column k.
     auto stage_half = [&](uint32_t chunk, int buffer) {
@@ -696,13 +702,13 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias,
         const uint64_t k0 = (uint64_t)tile0 * 128;
         // Aligned rows: one bulk copy each; the last eight columns, if not whole, by hand.
         const uint32_t whole = x_vec ? (uint32_t)(min((uint64_t)n16 * 8, w.k - k0) / 8) : 0;
-        if (threadIdx.x == 0) {
+        if (threadIdx.x == 0) qrc::mbar_arrive_expect_tx(x_bars + 8 * buffer, whole * 16 * tokens);
+        // Issuing a copy takes a thread about a tenth of a microsecond: the warps share them.
+        const int tok = warp + lane * W;
+        if (whole && tok < tokens) {
             qrc::fence_proxy_async_smem();                      // the buffer has been read: before its refill
-            qrc::mbar_arrive_expect_tx(x_bars + 8 * buffer, whole * 16 * tokens);
-            if (whole)
-                for (int tok = 0; tok < tokens; tok++)
-                    qrc::bulk_g2s(smem_at + (uint32_t)(to - smem) + tok * pitch, (uint64_t)(x + (m0 + tok) * ldx + k0),
-                                  whole * 16, x_bars + 8 * buffer);
+            qrc::bulk_g2s(smem_at + (uint32_t)(to - smem) + tok * pitch, (uint64_t)(x + (m0 + tok) * ldx + k0), whole * 16,
+                          x_bars + 8 * buffer);
         }
         const uint32_t rest = n16 - whole;
 #pragma unroll 4
@@ -772,7 +778,7 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias,
     uint32_t x_at[NT];
 #pragma unroll
     for (int i = 0; i < NT; i++) x_at[i] = min(i * 8 + g, columns - 1) * pitch;
-    const uint64_t u0 = units * blockIdx.x / gridDim.x, u1 = units * (blockIdx.x + 1) / gridDim.x;
+    const uint64_t u0 = row_tiles * blockIdx.x / gridDim.x, u1 = row_tiles * (blockIdx.x + 1) / gridDim.x;
     const uint32_t rows = (uint32_t)(u1 - u0), passes = (rows + W - 1) / W, per_pass = (rows + passes - 1) / passes;
     uint32_t parity = 0, x_parity = 0;
     bool failed = false, staged = false;
@@ -780,18 +786,11 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias,
         const uint32_t first = pass * per_pass, here = min(per_pass, rows - first);
         const uint32_t team = W / here, mine = warp / team, member = warp - mine * team;
         const bool active = mine < here;
-        const uint64_t unit = u0 + first + (active ? mine : 0);
-        const uint4* src[R];
-        const uint16_t* scale_at[R];
-        const uint8_t* zero_at[R];
-#pragma unroll
-        for (int r = 0; r < R; r++) {
-            // Rows behind the last one repeat it; their sums are not stored.
-            const uint64_t rt = min(unit * R + r, row_tiles - 1), row = min(rt * 16 + (lane & 15), w.n - 1);
-            src[r] = reinterpret_cast<const uint4*>(w.packed) + rt * tiles * 64;
-            scale_at[r] = static_cast<const uint16_t*>(w.scales) + row;
-            zero_at[r] = w.zeros + row;
-        }
+        // Rows behind the last one repeat it; their sums are not stored.
+        const uint64_t rt = u0 + first + (active ? mine : 0), my_row = min(rt * 16 + (lane & 15), w.n - 1);
+        const uint4* const src = reinterpret_cast<const uint4*>(w.packed) + rt * tiles * 64;
+        const uint16_t* const scale_at = static_cast<const uint16_t*>(w.scales) + my_row;
+        const uint8_t* const zero_at = w.zeros + my_row;
         // This warp's tile columns of a chunk: a run of them.
         auto run_of = [&](uint32_t chunk, uint32_t& lo, uint32_t& hi) {
             const uint32_t size = min(chunk_tiles, tiles - chunk * chunk_tiles);
@@ -813,38 +812,30 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias,
             const uint32_t n = min((uint32_t)BT, ahead_left);
             if (lane == 0) {
                 qrc::fence_proxy_async_smem();                  // the slot has been read: before its refill
-                qrc::mbar_arrive_expect_tx(bars + 8 * slot, n * R * 1024);
-#pragma unroll
-                for (int r = 0; r < R; r++)
-                    qrc::bulk_g2s(ring_at + slot * S::kSlot + r * BT * 1024, (uint64_t)(src[r] + (uint64_t)ahead_at * 64),
-                                  n * 1024, bars + 8 * slot);
+                qrc::mbar_arrive_expect_tx(bars + 8 * slot, n * 1024);
+                qrc::bulk_g2s(ring_at + slot * S::kSlot, (uint64_t)(src + (uint64_t)ahead_at * 64), n * 1024, bars + 8 * slot);
             }
             filled |= 1u << slot;
             ahead_at += n;
             ahead_left -= n;
             if (!ahead_left) settle();
         };
-        // Scales and zeros of a batch, one row and group per lane: those of
-        // row lane % 16 and group 2 * i + lane / 16 of a tile.
-        uint32_t scale[BT][R][kPer], zero[BT][R][kPer];
+        // Scales and zeros of a batch: a lane holds those of row lane % 16 and,
+        // counting the parts of its tiles that share a scale, part
+        // 2 * i + lane / 16.
+        uint32_t scale[kUnits], zero[kUnits];
         auto load_scales = [&](uint32_t tile) {
 #pragma unroll
-            for (int b = 0; b < BT; b++) {
-#pragma unroll
-                for (int i = 0; i < kPer; i++) {
-                    const uint32_t sub = SUB == 1 ? 0 : 2 * i + (lane >> 4);
-                    // Groups behind the last one repeat it: their sums are 0.
-                    const uint32_t group = min(SUB == 1 ? (tile + b) >> (w.group_log2 - 7) : (tile + b) * SUB + sub, groups - 1);
-#pragma unroll
-                    for (int r = 0; r < R; r++) {
-                        scale[b][r][i] = __ldg(scale_at[r] + (uint64_t)group * (uint32_t)w.n);
-                        if (ZEROS) zero[b][r][i] = __ldg(zero_at[r] + (uint64_t)group * (uint32_t)w.n);
-                    }
-                }
+            for (int i = 0; i < kUnits; i++) {
+                const uint32_t part = tile * SUB + 2 * i + (lane >> 4);
+                // Groups behind the last one repeat it: their sums are 0.
+                const uint32_t group = min(SUB == 1 ? part >> (w.group_log2 - 7) : part, groups - 1);
+                scale[i] = __ldg(scale_at + (uint64_t)group * (uint32_t)w.n);
+                if (ZEROS) zero[i] = __ldg(zero_at + (uint64_t)group * (uint32_t)w.n);
             }
         };
 
-        float sum[R][NT][4] = {};
+        float sum[NT][4] = {};
         settle();
         for (int i = 0; i < D && ahead_left && !failed; i++) fetch(i);
         int slot = 0;
@@ -872,105 +863,85 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias,
                 }
                 staged = true;
             }
-            const unsigned char* xt = xs + buffer * (columns * pitch) + lo * S::kRowBytes + t * 16;
-            const int4* it = info + lo * (SUB * NT * 4) + t;
-            for (uint32_t at = lo; at < hi; at += BT, xt += BT * S::kRowBytes, it += BT * SUB * NT * 4) {
-                uint32_t scale_now[BT][R][kPer], zero_now[BT][R][kPer];
+            uint32_t xt = smem_at + (uint32_t)(xs - smem) + buffer * (columns * pitch) + lo * S::kRowBytes + t * 16;
+            uint32_t it = smem_at + (uint32_t)(xs - smem) + columns * pitch + (lo * (SUB * NT * 4) + t) * 16;
+            for (uint32_t at = lo; at < hi; at += BT, xt += BT * S::kRowBytes, it += BT * SUB * NT * 64) {
+                uint32_t now[kUnits];                           // 8 * zero above the scale's bits
 #pragma unroll
-                for (int b = 0; b < BT; b++) {
-#pragma unroll
-                    for (int r = 0; r < R; r++) {
-#pragma unroll
-                        for (int i = 0; i < kPer; i++) {
-                            scale_now[b][r][i] = scale[b][r][i];
-                            if (ZEROS) zero_now[b][r][i] = zero[b][r][i];
-                        }
-                    }
-                }
+                for (int i = 0; i < kUnits; i++) now[i] = scale[i] | (ZEROS ? zero[i] : 8u) << 19;
                 if (at + BT < hi) load_scales(chunk * chunk_tiles + at + BT);
                 if (failed || !qrc::mbar_wait_bounded(bars + 8 * slot, (parity >> slot) & 1)) { failed = true; break; }
                 parity ^= 1u << slot;
                 filled &= ~(1u << slot);
-                const unsigned char* q = ring + slot * S::kSlot + lane * 16;
-                // Tile columns behind the run hold nothing of use: they are left out.
-#pragma unroll
-                for (int b = 0; b < BT; b++) {
-                    if (at + b >= hi) break;
-                    uint32_t top[R][4], low[R][4];
-#pragma unroll
-                    for (int r = 0; r < R; r++) {
-                        *reinterpret_cast<uint4*>(top[r]) = *reinterpret_cast<const uint4*>(q + (r * BT + b) * 1024);
-                        *reinterpret_cast<uint4*>(low[r]) = *reinterpret_cast<const uint4*>(q + (r * BT + b) * 1024 + 512);
-                    }
+                const uint32_t q = ring_at + slot * S::kSlot + lane * 16;
+                auto multiply = [&](int b) {
+                    const uint4 u = load_shared(q + b * 1024), l = load_shared(q + b * 1024 + 512);
+                    const uint32_t top[4] = {u.x, u.y, u.z, u.w}, low[4] = {l.x, l.y, l.z, l.w};
                     uint4 v[NT];
 #pragma unroll
                     for (int sub = 0; sub < SUB; sub++) {
-                        const int from = SUB == 1 ? 0 : (sub & 1) * 16;
-                        float sa[R], sb[R];
-                        uint32_t za[R], zb[R];
-#pragma unroll
-                        for (int r = 0; r < R; r++) {
-                            sa[r] = Half<T>::to_float(from_bits<T>(__shfl_sync(0xffffffffu, scale_now[b][r][sub / 2], from + g)));
-                            sb[r] = Half<T>::to_float(from_bits<T>(__shfl_sync(0xffffffffu, scale_now[b][r][sub / 2], from + g + 8)));
-                            za[r] = ZEROS ? __shfl_sync(0xffffffffu, zero_now[b][r][sub / 2], from + g) * 8 : 64u;
-                            zb[r] = ZEROS ? __shfl_sync(0xffffffffu, zero_now[b][r][sub / 2], from + g + 8) * 8 : 64u;
-                            if (!DIGITS) {
-                                za[r] = za[r] * 0x10001u | Half<T>::kOne;
-                                zb[r] = zb[r] * 0x10001u | Half<T>::kOne;
-                            }
-                        }
-                        Sum part[R][NT][4] = {};
+                        const int part_at = (b * SUB + sub) / 2, from = (b * SUB + sub) % 2 * 16 + g;
+                        const uint32_t pa = __shfl_sync(0xffffffffu, now[part_at], from), pb = __shfl_sync(0xffffffffu, now[part_at], from + 8);
+                        const float sa = Half<T>::to_float(from_bits<T>(pa)), sb = Half<T>::to_float(from_bits<T>(pb));
+                        // the zeros as whole numbers, or as code_pair forms codes
+                        const uint32_t za = DIGITS ? pa >> 16 : __byte_perm(pa, 0, 0x3232) | Half<T>::kOne;
+                        const uint32_t zb = DIGITS ? pb >> 16 : __byte_perm(pb, 0, 0x3232) | Half<T>::kOne;
+                        Sum part[NT][4] = {};
 #pragma unroll
                         for (int j = sub * 4 / SUB; j < (sub + 1) * 4 / SUB; j++) {
 #pragma unroll
                             for (int i = 0; i < NT; i++) {
-                                if (!DIGITS) v[i] = *reinterpret_cast<const uint4*>(xt + x_at[i] + b * 256 + j * 64);
-                                else if (j % 2 == 0) v[i] = *reinterpret_cast<const uint4*>(xt + x_at[i] + b * 128 + j * 32);
+                                if (!DIGITS) v[i] = load_shared(xt + x_at[i] + b * 256 + j * 64);
+                                else if (j % 2 == 0) v[i] = load_shared(xt + x_at[i] + b * 128 + j * 32);
                             }
+                            if constexpr (DIGITS) {
+                                const uint32_t a[4] = {top[j] & 0x78787878u, low[j] & 0x78787878u,
+                                                       rotate_right(top[j], 4) & 0x78787878u, rotate_right(low[j], 4) & 0x78787878u};
 #pragma unroll
-                            for (int r = 0; r < R; r++) {
-                                const uint32_t wt = top[r][j], wl = low[r][j];
-                                if constexpr (DIGITS) {
-                                    const uint32_t a[4] = {wt & 0x78787878u, wl & 0x78787878u,
-                                                           rotate_right(wt, 4) & 0x78787878u, rotate_right(wl, 4) & 0x78787878u};
+                                for (int i = 0; i < NT; i++)
+                                    mma_bytes(part[i], a, j % 2 ? v[i].z : v[i].x, j % 2 ? v[i].w : v[i].y);
+                            } else {
+                                uint32_t a[2][4];
 #pragma unroll
-                                    for (int i = 0; i < NT; i++) mma_bytes(part[r][i], a, j % 2 ? v[i].z : v[i].x, j % 2 ? v[i].w : v[i].y);
-                                } else {
-                                    uint32_t a[2][4];
-#pragma unroll
-                                    for (int h = 0; h < 2; h++) {
-                                        a[h][0] = Half<T>::sub2(code_pair<T>(wt, 2 * h), za[r]);
-                                        a[h][1] = Half<T>::sub2(code_pair<T>(wl, 2 * h), zb[r]);
-                                        a[h][2] = Half<T>::sub2(code_pair<T>(wt, 2 * h + 1), za[r]);
-                                        a[h][3] = Half<T>::sub2(code_pair<T>(wl, 2 * h + 1), zb[r]);
-                                    }
-#pragma unroll
-                                    for (int i = 0; i < NT; i++) {
-                                        Half<T>::mma(part[r][i], a[0], v[i].x, v[i].y);
-                                        Half<T>::mma(part[r][i], a[1], v[i].z, v[i].w);
-                                    }
+                                for (int h = 0; h < 2; h++) {
+                                    a[h][0] = Half<T>::sub2(code_pair<T>(top[j], 2 * h), za);
+                                    a[h][1] = Half<T>::sub2(code_pair<T>(low[j], 2 * h), zb);
+                                    a[h][2] = Half<T>::sub2(code_pair<T>(top[j], 2 * h + 1), za);
+                                    a[h][3] = Half<T>::sub2(code_pair<T>(low[j], 2 * h + 1), zb);
                                 }
+#pragma unroll
+                                for (int i = 0; i < NT; i++) Half<T>::mma(part[i], a[0], v[i].x, v[i].y);
+#pragma unroll
+                                for (int i = 0; i < NT; i++) Half<T>::mma(part[i], a[1], v[i].z, v[i].w);
                             }
                         }
 #pragma unroll
                         for (int i = 0; i < NT; i++) {
-                            int4 of = make_int4(0, 0, 0, 0);
-                            if (DIGITS) of = it[((b * SUB + sub) * NT + i) * 4];
+                            if constexpr (DIGITS) {
+                                const uint4 of = load_shared(it + ((b * SUB + sub) * NT + i) * 64);
+                                const float f[2] = {__uint_as_float(of.z), __uint_as_float(of.w)};
+                                const int digits[2] = {(int)of.x, (int)of.y};
 #pragma unroll
-                            for (int r = 0; r < R; r++) {
-                                if constexpr (DIGITS) {
-                                    const float f0 = __int_as_float(of.z), f1 = __int_as_float(of.w);
-                                    sum[r][i][0] = fmaf(sa[r] * f0, (float)(part[r][i][0] - (int)za[r] * of.x), sum[r][i][0]);
-                                    sum[r][i][1] = fmaf(sa[r] * f1, (float)(part[r][i][1] - (int)za[r] * of.y), sum[r][i][1]);
-                                    sum[r][i][2] = fmaf(sb[r] * f0, (float)(part[r][i][2] - (int)zb[r] * of.x), sum[r][i][2]);
-                                    sum[r][i][3] = fmaf(sb[r] * f1, (float)(part[r][i][3] - (int)zb[r] * of.y), sum[r][i][3]);
-                                } else {
-                                    add_scaled<NT>(sum[r][i][0], sum[r][i][1], sa[r], part[r][i][0], part[r][i][1]);
-                                    add_scaled<NT>(sum[r][i][2], sum[r][i][3], sb[r], part[r][i][2], part[r][i][3]);
+                                for (int e = 0; e < 4; e++) {
+                                    const int whole = part[i][e] - (int)(e < 2 ? za : zb) * digits[e & 1];
+                                    sum[i][e] = fmaf((e < 2 ? sa : sb) * f[e & 1], (float)whole, sum[i][e]);
                                 }
+                            } else {
+                                add_scaled<NT>(sum[i][0], sum[i][1], sa, part[i][0], part[i][1]);
+                                add_scaled<NT>(sum[i][2], sum[i][3], sb, part[i][2], part[i][3]);
                             }
                         }
                     }
+                };
+                // A whole batch without a check in between: the checks cost a sixth
+                // of the instructions.  Tile columns behind the run are left out.
+                if (at + BT <= hi) {
+#pragma unroll
+                    for (int b = 0; b < BT; b++) multiply(b);
+                } else {
+#pragma unroll
+                    for (int b = 0; b < BT - 1; b++)
+                        if (at + b < hi) multiply(b);
                 }
                 __syncwarp();
                 if (ahead_left) fetch(slot);
@@ -986,28 +957,24 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias,
         }
 
         // The sums of a team meet in its slots, which hold nothing any more.
-        float* const out = reinterpret_cast<float*>(ring);      // [8 * NT][16 * R]
+        float* const out = reinterpret_cast<float*>(ring);      // [8 * NT][16]
         if (active) {
 #pragma unroll
-            for (int r = 0; r < R; r++) {
+            for (int i = 0; i < NT; i++) {
 #pragma unroll
-                for (int i = 0; i < NT; i++) {
-#pragma unroll
-                    for (int e = 0; e < 4; e++) out[(i * 8 + 2 * t + (e & 1)) * (16 * R) + r * 16 + g + (e >> 1) * 8] = sum[r][i][e];
-                }
+                for (int e = 0; e < 4; e++) out[(i * 8 + 2 * t + (e & 1)) * 16 + g + (e >> 1) * 8] = sum[i][e];
             }
         }
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < here * tokens * 16 * R; i += W * 32) {
-            const uint32_t r = i % (16 * R), tok = i / (16 * R) % tokens, which = i / (16 * R * tokens);
-            const uint64_t row = (u0 + first + which) * 16 * R + r;
+        for (uint32_t i = threadIdx.x; i < here * tokens * 16; i += W * 32) {
+            const uint32_t r = i % 16, tok = i / 16 % tokens, which = i / (16 * tokens);
+            const uint64_t row = (u0 + first + which) * 16 + r;
             if (row >= w.n) continue;
             float v[S::kColumns] = {};
             for (uint32_t j = 0; j < team; j++) {
-                const float* part = reinterpret_cast<const float*>(smem + (which * team + j) * (D * S::kSlot)) +
-                                    tok * S::kColumns * (16 * R) + r;
+                const float* part = reinterpret_cast<const float*>(smem + (which * team + j) * (D * S::kSlot)) + tok * S::kColumns * 16 + r;
 #pragma unroll
-                for (int p = 0; p < S::kColumns; p++) v[p] += part[p * (16 * R)];
+                for (int p = 0; p < S::kColumns; p++) v[p] += part[p * 16];
             }
             float all = v[0] * (DIGITS ? 65536.0f : 1.0f / Half<T>::kUnit);
             if constexpr (DIGITS) all += v[1] * 256.0f + v[2];
@@ -1069,14 +1036,14 @@ int launch_shape(const qrc_w4& w, const T* x, uint64_t ldx, uint64_t m, const T*
                  int y_float, int sms, cudaStream_t s) {
     const W4 a = {w.d_packed, w.d_scales, w.d_zeros, w.n, w.k, log2_of(w.group)};
     const int x_vec = rows_aligned(x, ldx, m, 2), sub = w.group == 32 ? 4 : w.group == 64 ? 2 : 1;
-    const uint64_t tiles = (w.k + 127) / 128, units = ((w.n + 15) / 16 + S::R - 1) / S::R;
+    const uint64_t tiles = (w.k + 127) / 128, row_tiles = (w.n + 15) / 16;
     const uint64_t tokens = std::min<uint64_t>(m, S::kTokens);
     // As many columns at a time as fit beside the ring, in chunks of one size.
     const uint64_t most = (kSmemLimit - S::fixed(tokens)) / S::per_tile(tokens, sub);
     const uint64_t chunks = std::max<uint64_t>((tiles + most - 1) / most, 1);
     const uint32_t chunk_tiles = (uint32_t)std::max<uint64_t>((tiles + chunks - 1) / chunks, 1);
     const size_t smem = S::fixed(tokens) + chunk_tiles * S::per_tile(tokens, sub);
-    const dim3 grid((unsigned)std::min<uint64_t>(units, sms), (unsigned)((m + S::kTokens - 1) / S::kTokens));
+    const dim3 grid((unsigned)std::min<uint64_t>(row_tiles, sms), (unsigned)((m + S::kTokens - 1) / S::kTokens));
     auto go = [&](auto kernel) -> int {
         QRC_CK(grant_smem((const void*)kernel, kSmemLimit));
         QRC_CK(launch_overlapped(kernel, grid, S::W * 32, smem, s, 1, a, x, ldx, m, bias, y, ldy, y_float, x_vec, chunk_tiles));
@@ -1100,9 +1067,9 @@ int launch_matvec(const qrc_w4& w, const void* d_x, uint64_t m, uint64_t ldx, co
         const T* x = static_cast<const T*>(d_x) + m0 * ldx;
         void* y = static_cast<char*>(d_y) + m0 * ldy * (y_float ? 4 : 2);
         auto go = [&](auto shape) { return launch_shape<T, decltype(shape)>(w, x, ldx, rows, bias, y, ldy, y_float, sms, s); };
-        const int rc = rows <= 2 ? go(Shape<true, 1, 16, 1, 4, 2>())
-                       : rows <= 8 ? go(Shape<false, 1, 16, 1, 4, 2>())
-                       : rows <= 16 ? go(Shape<false, 2, 16, 1, 4, 2>()) : go(Shape<false, 4, 8, 2, 2, 2>());
+        const int rc = rows <= 2 ? go(Shape<true, 1, 16, 4, 2>())
+                       : rows <= 8 ? go(Shape<false, 1, 16, 4, 2>())
+                       : rows <= 16 ? go(Shape<false, 2, 12, 4, 2>()) : go(Shape<false, 4, 8, 4, 2>());
         if (rc != QRC_OK) return rc;
     }
     return QRC_OK;
