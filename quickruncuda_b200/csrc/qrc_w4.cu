@@ -596,6 +596,22 @@ __device__ __forceinline__ uint4 load_shared(uint32_t at) {
     return v;
 }
 
+// A word of shared memory of block `from` of the cluster, at the address it
+// has in this one, block `rank`.
+__device__ __forceinline__ uint32_t peer_word(uint32_t at, uint32_t from, uint32_t rank) {
+    uint32_t there, v;
+    if (from == rank) {
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+        return v;
+    }
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(from));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(there) : "memory");
+    return v;
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 __device__ __forceinline__ void mma_bytes(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
@@ -613,15 +629,14 @@ struct Shape {
     static constexpr int kColumns = DIGITS ? 3 : 1;                     // matrix columns of one of them
     static constexpr int kRowBytes = DIGITS ? 128 : 256;                // of a column, per tile
     static constexpr int kSlot = BT * 1024;                             // bytes
-    static constexpr int kRing = W * D * kSlot, kBars = W * D * 8 + 16;
-    static constexpr int kBuffers = DIGITS ? 1 : 2;                     // chunks of activations held
+    static constexpr int kRing = W * D * kSlot, kBars = W * D * 8 + 32;     // the last 16 bytes: whether a wait gave up
     static_assert(16 * 8 * NT * 4 <= D * kSlot, "a warp's sums have to fit in its slots");
     // Shared memory a tile column of activations takes, and what does not
     // depend on their number.
-    static constexpr uint64_t per_tile(uint64_t tokens, int sub) {
-        return kBuffers * tokens * kColumns * kRowBytes + (DIGITS ? sub * NT * 64 : 0);
+    static constexpr uint64_t per_tile(uint64_t tokens, int sub, int buffers) {
+        return buffers * tokens * kColumns * kRowBytes + (DIGITS ? sub * NT * 64 : 0);
     }
-    static constexpr uint64_t fixed(uint64_t tokens) { return kRing + kBars + kBuffers * tokens * kColumns * 64; }
+    static constexpr uint64_t fixed(uint64_t tokens, int buffers) { return kRing + kBars + buffers * tokens * kColumns * 64; }
 };
 
 // y = values * x for the rows of tiles of this block.
@@ -651,18 +666,21 @@ struct Shape {
 template <class T, class S, int SUB, bool ZEROS>
 __global__ void __launch_bounds__(S::W * 32, 1)
 qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias, void* y, uint64_t ldy, int y_float,
-                int x_vec, uint32_t chunk_tiles) {
+                int x_vec, uint32_t chunk_tiles, uint32_t cluster) {
     constexpr bool DIGITS = S::DIGITS;
     constexpr int NT = S::NT, W = S::W, BT = S::BT, D = S::D, kUnits = BT * SUB / 2;
     using Sum = std::conditional_t<DIGITS, int, float>;
     extern __shared__ __align__(16) unsigned char smem[];
-    __shared__ int s_failed;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const uint64_t m0 = (uint64_t)blockIdx.y * S::kTokens;
     const int tokens = (int)min((uint64_t)S::kTokens, m - m0), columns = tokens * S::kColumns;
     const uint32_t tiles = (uint32_t)((w.k + 127) / 128);
     const uint32_t groups = (uint32_t)((w.k + (1ull << w.group_log2) - 1) >> w.group_log2);
-    const uint32_t chunks = (tiles + chunk_tiles - 1) / chunk_tiles;
+    // This block's share of the columns, and its chunks.
+    const uint32_t rank = blockIdx.x % cluster, tile_lo = (uint64_t)tiles * rank / cluster;
+    const uint32_t tile_hi = (uint64_t)tiles * (rank + 1) / cluster, chunks = (tile_hi - tile_lo + chunk_tiles - 1) / chunk_tiles;
+    auto tile_of = [&](uint32_t chunk) { return tile_lo + chunk * chunk_tiles; };
+    auto size_of = [&](uint32_t chunk) { return min(chunk_tiles, tile_hi - tile_of(chunk)); };
     const uint64_t row_tiles = (w.n + 15) / 16;
     const uint32_t pitch = chunk_tiles * S::kRowBytes + 64;     // columns of activations, apart in the banks
     unsigned char* const ring = smem + warp * (D * S::kSlot);
@@ -673,8 +691,11 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias,
     // DIGITS: per tile, group and pair of columns, the digits' sums and the unit of x
     int4* const info = reinterpret_cast<int4*>(xs + columns * pitch);
 
+    volatile uint32_t* const failed_word = reinterpret_cast<uint32_t*>(smem + S::kRing + W * D * 8 + 16);
+    auto sync_all = [&]() { if (cluster > 1) cluster_barrier(); else __syncthreads(); };
+
     if (threadIdx.x == 0) {
-        s_failed = 0;
+        *failed_word = 0;
         qrc::mbar_init(x_bars, 1);
         qrc::mbar_init(x_bars + 8, 1);
     }
@@ -697,7 +718,7 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias,
     };
     // Brings a chunk's activations to shared memory, zero behind column k.
     auto stage_half = [&](uint32_t chunk, int buffer) {
-        const uint32_t tile0 = chunk * chunk_tiles, n16 = min(chunk_tiles, tiles - tile0) * 16;
+        const uint32_t tile0 = tile_of(chunk), n16 = size_of(chunk) * 16;
         unsigned char* const to = xs + buffer * (columns * pitch);
         const uint64_t k0 = (uint64_t)tile0 * 128;
         // Aligned rows: one bulk copy each; the last eight columns, if not whole, by hand.
@@ -719,7 +740,7 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias,
     };
     // The same as three bytes per activation, with the sums of the bytes.
     auto stage_digits = [&](uint32_t chunk) {
-        const uint32_t tile0 = chunk * chunk_tiles, n16 = min(chunk_tiles, tiles - tile0) * 16, padded = (n16 + 31) / 32 * 32;
+        const uint32_t tile0 = tile_of(chunk), n16 = size_of(chunk) * 16, padded = (n16 + 31) / 32 * 32;
         constexpr int kLanes = 16 / SUB;                        // lanes of a group, eight columns each
         // Whole warps take part, and a group lies within one: rows are padded to 32 lanes.
         for (uint32_t i = threadIdx.x; i < padded * tokens; i += W * 32) {
@@ -778,7 +799,8 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias,
     uint32_t x_at[NT];
 #pragma unroll
     for (int i = 0; i < NT; i++) x_at[i] = min(i * 8 + g, columns - 1) * pitch;
-    const uint64_t u0 = row_tiles * blockIdx.x / gridDim.x, u1 = row_tiles * (blockIdx.x + 1) / gridDim.x;
+    const uint32_t group_of = blockIdx.x / cluster, groups_of = gridDim.x / cluster;
+    const uint64_t u0 = row_tiles * group_of / groups_of, u1 = row_tiles * (group_of + 1) / groups_of;
     const uint32_t rows = (uint32_t)(u1 - u0), passes = (rows + W - 1) / W, per_pass = (rows + passes - 1) / passes;
     uint32_t parity = 0, x_parity = 0;
     bool failed = false, staged = false;
@@ -793,7 +815,7 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias,
         const uint8_t* const zero_at = w.zeros + my_row;
         // This warp's tile columns of a chunk: a run of them.
         auto run_of = [&](uint32_t chunk, uint32_t& lo, uint32_t& hi) {
-            const uint32_t size = min(chunk_tiles, tiles - chunk * chunk_tiles);
+            const uint32_t size = size_of(chunk);
             lo = active ? size * member / team : 0;
             hi = active ? size * (member + 1) / team : 0;
         };
@@ -803,7 +825,7 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias,
             while (ahead_left == 0 && ahead_chunk < chunks) {
                 uint32_t lo, hi;
                 run_of(ahead_chunk, lo, hi);
-                ahead_at = ahead_chunk * chunk_tiles + lo;
+                ahead_at = tile_of(ahead_chunk) + lo;
                 ahead_left = hi - lo;
                 ahead_chunk++;
             }
@@ -846,7 +868,7 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias,
         for (uint32_t chunk = 0; chunk < chunks; chunk++) {
             uint32_t lo, hi;
             run_of(chunk, lo, hi);
-            if (lo < hi) load_scales(chunk * chunk_tiles + lo);
+            if (lo < hi) load_scales(tile_of(chunk) + lo);
             const int buffer = DIGITS ? 0 : chunk & 1;
             if (!staged || chunks > 1) {
                 if (DIGITS) {
@@ -869,7 +891,7 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias,
                 uint32_t now[kUnits];                           // 8 * zero above the scale's bits
 #pragma unroll
                 for (int i = 0; i < kUnits; i++) now[i] = scale[i] | (ZEROS ? zero[i] : 8u) << 19;
-                if (at + BT < hi) load_scales(chunk * chunk_tiles + at + BT);
+                if (at + BT < hi) load_scales(tile_of(chunk) + at + BT);
                 if (failed || !qrc::mbar_wait_bounded(bars + 8 * slot, (parity >> slot) & 1)) { failed = true; break; }
                 parity ^= 1u << slot;
                 filled &= ~(1u << slot);
@@ -949,7 +971,7 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias,
             }
         }
         if (failed) {                                           // a wait gave up: wait, bounded, for what is under way
-            s_failed = 1;
+            *failed_word = 1;
             for (int i = 0; i < D; i++)
                 if (filled >> i & 1) qrc::mbar_wait_bounded(bars + 8 * i, (parity >> i) & 1);
             filled = 0;
@@ -965,25 +987,29 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias,
                 for (int e = 0; e < 4; e++) out[(i * 8 + 2 * t + (e & 1)) * 16 + g + (e >> 1) * 8] = sum[i][e];
             }
         }
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < here * tokens * 16; i += W * 32) {
+        sync_all();
+        for (uint32_t i = threadIdx.x + rank * (W * 32); i < here * tokens * 16; i += W * 32 * cluster) {
             const uint32_t r = i % 16, tok = i / 16 % tokens, which = i / (16 * tokens);
             const uint64_t row = (u0 + first + which) * 16 + r;
             if (row >= w.n) continue;
             float v[S::kColumns] = {};
-            for (uint32_t j = 0; j < team; j++) {
-                const float* part = reinterpret_cast<const float*>(smem + (which * team + j) * (D * S::kSlot)) + tok * S::kColumns * 16 + r;
+            bool bad = false;
+            for (uint32_t from = 0; from < cluster; from++) {
+                bad = bad || peer_word(smem_at + S::kRing + W * D * 8 + 16, from, rank) != 0;
+                for (uint32_t j = 0; j < team; j++) {
+                    const uint32_t part = smem_at + (which * team + j) * (D * S::kSlot) + (tok * S::kColumns * 16 + r) * 4;
 #pragma unroll
-                for (int p = 0; p < S::kColumns; p++) v[p] += part[p * 16];
+                    for (int p = 0; p < S::kColumns; p++) v[p] += __uint_as_float(peer_word(part + p * 64, from, rank));
+                }
             }
             float all = v[0] * (DIGITS ? 65536.0f : 1.0f / Half<T>::kUnit);
             if constexpr (DIGITS) all += v[1] * 256.0f + v[2];
             if (bias) all += Half<T>::to_float(bias[row]);
-            if (s_failed) all = __int_as_float(0x7fffffff);     // NaN: no valid result
+            if (bad) all = __int_as_float(0x7fffffff);          // a wait gave up: no valid result
             if (y_float) static_cast<float*>(y)[(m0 + tok) * ldy + row] = all;
             else static_cast<T*>(y)[(m0 + tok) * ldy + row] = Half<T>::round(all);
         }
-        if (pass + 1 < passes) __syncthreads();                 // before the slots are filled again
+        if (pass + 1 < passes || cluster > 1) sync_all();       // before the slots are filled again, or gone
     }
 }
 
@@ -1028,8 +1054,7 @@ dim3 grid_for(uint64_t items, uint64_t per_block) {
     return dim3((unsigned)std::min<uint64_t>((items + per_block - 1) / per_block, 1u << 20));
 }
 
-// Shared memory a block may have, and what its static part takes.
-constexpr int kSmemLimit = 227 * 1024 - 64;
+constexpr int kSmemLimit = 227 * 1024;        // a block's shared memory
 
 template <class T, class S>
 int launch_shape(const qrc_w4& w, const T* x, uint64_t ldx, uint64_t m, const T* bias, void* y, uint64_t ldy,
@@ -1038,15 +1063,25 @@ int launch_shape(const qrc_w4& w, const T* x, uint64_t ldx, uint64_t m, const T*
     const int x_vec = rows_aligned(x, ldx, m, 2), sub = w.group == 32 ? 4 : w.group == 64 ? 2 : 1;
     const uint64_t tiles = (w.k + 127) / 128, row_tiles = (w.n + 15) / 16;
     const uint64_t tokens = std::min<uint64_t>(m, S::kTokens);
-    // As many columns at a time as fit beside the ring, in chunks of one size.
-    const uint64_t most = (kSmemLimit - S::fixed(tokens)) / S::per_tile(tokens, sub);
-    const uint64_t chunks = std::max<uint64_t>((tiles + most - 1) / most, 1);
-    const uint32_t chunk_tiles = (uint32_t)std::max<uint64_t>((tiles + chunks - 1) / chunks, 1);
-    const size_t smem = S::fixed(tokens) + chunk_tiles * S::per_tile(tokens, sub);
-    const dim3 grid((unsigned)std::min<uint64_t>(row_tiles, sms), (unsigned)((m + S::kTokens - 1) / S::kTokens));
+    // Rows are split between the SMs; or between pairs of them, clusters of two
+    // blocks with half of the columns each, where that leaves the busiest block
+    // a tenth less to do (5003 x 11007 with 5 rows: 22 us, without 28; with
+    // even shares the pair's barriers cost more: 4096 x 4096 6.8 us, 6.0).
+    const uint64_t alone = (row_tiles + sms - 1) / sms * tiles;
+    const uint64_t paired = (row_tiles + sms / 2 - 1) / (sms / 2) * ((tiles + 1) / 2);
+    const int cluster = sms % 2 == 0 && paired * 10 <= alone * 9 ? 2 : 1;
+    const uint64_t share = (tiles + cluster - 1) / cluster;
+    // All of a block's columns at once where they fit beside the ring, else
+    // chunks of one size, two at a time.
+    auto fitting = [&](int buffers) { return (kSmemLimit - S::fixed(tokens, buffers)) / S::per_tile(tokens, sub, buffers); };
+    const int buffers = S::DIGITS || share <= fitting(1) ? 1 : 2;
+    const uint64_t chunks = std::max<uint64_t>((share + fitting(buffers) - 1) / fitting(buffers), 1);
+    const uint32_t chunk_tiles = (uint32_t)std::max<uint64_t>((share + chunks - 1) / chunks, 1);
+    const size_t smem = S::fixed(tokens, buffers) + chunk_tiles * S::per_tile(tokens, sub, buffers);
+    const dim3 grid((unsigned)std::min<uint64_t>(row_tiles, sms / cluster) * cluster, (unsigned)((m + S::kTokens - 1) / S::kTokens));
     auto go = [&](auto kernel) -> int {
         QRC_CK(grant_smem((const void*)kernel, kSmemLimit));
-        QRC_CK(launch_overlapped(kernel, grid, S::W * 32, smem, s, 1, a, x, ldx, m, bias, y, ldy, y_float, x_vec, chunk_tiles));
+        QRC_CK(launch_overlapped(kernel, grid, S::W * 32, smem, s, cluster, a, x, ldx, m, bias, y, ldy, y_float, x_vec, chunk_tiles, cluster));
         return QRC_OK;
     };
     switch (sub) {
