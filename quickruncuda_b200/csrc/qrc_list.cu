@@ -638,6 +638,19 @@ cudaError_t norm_by_order(const qrc_list& l, int norm, double* work, float* d_no
     }
 }
 
+// Whether a float lies within an output's first and last byte.
+bool covers(const qrc_list& l, const float* p) {
+    const uint64_t at = (uintptr_t)p;
+    for (const Launch& a : l.launches) {
+        for (const Entry& e : a.entries) {
+            const uint64_t n = e.n_kind & ((1ull << kKindShift) - 1), out = (uintptr_t)e.out;
+            const uint64_t span = e.cols ? (n / e.cols - 1) * e.out_pitch + e.cols : n;
+            if (at + 4 > out && at < out + span * elem_bytes((int)(e.n_kind >> (kKindShift + 4)))) return true;
+        }
+    }
+    return false;
+}
+
 bool known_type(int t) { return t == QRC_F32 || t == QRC_BF16 || t == QRC_F16; }
 bool known_norm(int n) { return n == QRC_NORM_1 || n == QRC_NORM_2 || n == QRC_NORM_INF; }
 
@@ -732,6 +745,7 @@ QRC_API int qrc_list_clip(const qrc_list* l, int norm, double max_norm, const fl
         QRC_CK(small_by_order(*l, norm, d_norm, 1, max_norm, s));
         return QRC_OK;
     }
+    if (d_given && covers(*l, d_given)) return QRC_ERR_INVALID;
     double* work = static_cast<double*>(d_work);
     // Few partial results: the scale pass adds them up, without a launch for it.
     const bool fold = !d_given && l->launches.size() == 1 && l->partials <= kFold;

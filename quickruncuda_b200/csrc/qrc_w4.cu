@@ -406,6 +406,8 @@ qrc_k_w4_quant(const uint16_t* w, uint64_t ld, uint64_t n, uint64_t k, uint32_t*
 
 // -- pack and dequantize -----------------------------------------------------------
 
+// A thread per word.  VEC: eight codes in one load.
+template <bool VEC>
 __global__ void __launch_bounds__(256)
 qrc_k_w4_pack(const uint8_t* codes, uint64_t ld, uint64_t n, uint64_t k, uint32_t* packed) {
     qrc::griddep_wait();
@@ -414,10 +416,17 @@ qrc_k_w4_pack(const uint8_t* codes, uint64_t ld, uint64_t n, uint64_t k, uint32_
     for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) {
         const uint64_t tile = i >> 8, above = tile / tiles;
         const uint64_t row = above * 16 + ((i >> 4) & 15), col = (tile - above * tiles) * 128 + word_column(i & 15);
+        const uint8_t* const p = codes + row * ld + col;
         uint32_t word = 0;
+        if (VEC && row < n && col + 8 <= k) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
 #pragma unroll
-        for (int e = 0; e < 8; e++)
-            if (row < n && col + e < k) word |= place_code(codes[row * ld + col + e] & 15u, e);
+            for (int e = 0; e < 8; e++) word |= place_code((e < 4 ? v.x >> 8 * e : v.y >> 8 * (e - 4)) & 15u, e);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (row < n && col + e < k) word |= place_code(p[e] & 15u, e);
+        }
         packed[i] = word;
     }
 }
@@ -1182,7 +1191,8 @@ QRC_API int qrc_w4_pack(int device, const uint8_t* d_codes, uint64_t ld, const q
     if (!w->n || !w->k) return QRC_OK;
     DeviceScope scope(device);
     if (!scope.ok) return QRC_ERR_DEVICE;
-    QRC_CK(launch_overlapped(qrc_k_w4_pack, grid_for(qrc_w4_words(w->n, w->k), 256), 256, 0, as_stream(stream), 1,
+    const bool vec = !((uintptr_t)d_codes & 7) && (w->n <= 1 || ld % 8 == 0);
+    QRC_CK(launch_overlapped(vec ? qrc_k_w4_pack<true> : qrc_k_w4_pack<false>, grid_for(qrc_w4_words(w->n, w->k), 256), 256, 0, as_stream(stream), 1,
                              d_codes, ld, w->n, w->k, w->d_packed));
     return QRC_OK;
 }

@@ -138,6 +138,8 @@ class Weight4:
         n, k = self.shape
         if x.dtype is not self.dtype or x.device != self.device:
             _check(x, "x", (self.dtype,), device=self.device)
+        if x.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("Weight4: matvec has no backward pass; call it under torch.no_grad() or on x.detach()")
         shape = x.shape
         if not shape or shape[-1] != k:
             raise RuntimeError(f"Weight4: x has shape {tuple(shape)}, needs [..., {k}]")

@@ -327,3 +327,54 @@ def test_operators(cuda, qrc):
     _check_norm(n, x[:2], 2.0)
     _check_clip([a, b], x[:2], 0.25, 2.0)
     assert torch.equal(twice, a * 2)
+
+
+def test_given_norm_inside_an_output_is_refused(cuda, qrc):
+    import torch
+    x = torch.ones(100, device=cuda)
+    t = qrc.TensorList([x])
+    with pytest.raises(qrc.QrcError):
+        t.clip_norm(1.0, norm=x[50])
+    t.clip_norm(1.0, norm=torch.full((), 2.0, device=cuda))
+    assert (x - 0.5).abs().max() < 1e-6
+
+
+def test_c_workspace_is_required(cuda, qrc, lib):
+    import torch
+    x = torch.ones(1 << 20, device=cuda)
+    t = qrc.TensorList([x])
+    out = torch.empty(1, device=cuda)
+    need = lib.qrc_list_workspace(t.handle)
+    assert need > 0
+    work = torch.empty(need + 8, dtype=torch.uint8, device=cuda)
+    s = torch.cuda.current_stream().cuda_stream
+    assert lib.qrc_list_norm(t.handle, 2, out.data_ptr(), None, s) == -1
+    assert lib.qrc_list_norm(t.handle, 2, out.data_ptr(), work.data_ptr() + 4, s) == -1
+    assert lib.qrc_list_norm(t.handle, 3, out.data_ptr(), work.data_ptr(), s) == -1
+    assert lib.qrc_list_clip(t.handle, 2, 1.0, None, out.data_ptr(), None, s) == -1
+    assert lib.qrc_list_clip(t.handle, 2, -1.0, None, out.data_ptr(), work.data_ptr(), s) == -1
+    work.fill_(255)                                            # its contents do not matter
+    assert lib.qrc_list_norm(t.handle, 2, out.data_ptr(), work.data_ptr(), s) == 0
+    assert float(out) == 1024.0
+    norms = qrc.TensorList([x], out=[torch.empty_like(x)])      # a list that only some calls write through
+    assert float(norms.norm(1.0)) == 2.0 ** 20
+
+
+@pytest.mark.slow
+def test_more_than_2_to_32_elements(cuda, qrc):
+    import torch
+    n = (1 << 32) + 8192 + 3
+    x = torch.ones(n, dtype=torch.float16, device=cuda)
+    x[-3] = 9.0
+    t = qrc.TensorList([x[1:], x[:1]])
+    assert float(t.norm(1.0)) == torch.tensor(float(n + 8)).item()
+    assert float(t.norm(math.inf)) == 9.0
+    norm = float(t.clip_norm(4.5, math.inf))
+    assert norm == 9.0 and float(x[-3]) == 4.5 and float(x[0]) == float(x[n // 2]) == float(x[-1]) == 0.5
+    assert int((x != 0.5).sum()) == 1
+    # rows at one distance, the last one beyond 2^32
+    v = x[:(1 << 32) + 8192].view(-1, 8192)[:, 8:16]
+    u = qrc.TensorList([v])
+    assert float(u.norm(1.0)) == v.numel() * 0.5
+    u.clip_norm(0.0)
+    assert int((x == 0).sum()) == v.numel()

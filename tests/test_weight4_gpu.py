@@ -332,3 +332,67 @@ def test_operators(cuda, qrc):
             packed, values, y = g(w, x)
             assert torch.equal(packed, a.packed) and torch.equal(values, a.dequant())
             assert torch.equal(y, a.matvec(x, out_dtype=torch.float32))
+
+
+def test_backward_is_refused(cuda, qrc):
+    import torch
+    w4 = qrc.quant_w4(torch.randn(16, 64, device=cuda).half())
+    x = torch.randn(2, 64, device=cuda).half().requires_grad_()
+    with pytest.raises(RuntimeError, match="backward"):
+        w4.matvec(x)
+    with torch.no_grad():
+        assert torch.equal(w4.matvec(x), w4.matvec(x.detach()))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_matvec_activations_of_any_size(cuda, qrc, kind):
+    """One and two rows go through whole numbers scaled per group: ranges that
+    differ from group to group, zeros, the type's ends."""
+    import torch
+    n, k, group = 96, 1000, 32
+    codes, scales, zeros, gen = _case(cuda, n, k, kind, group, False, spread=False)
+    w4 = qrc.Weight4.from_codes(codes, scales, zeros, group=group)
+    values = _values(codes, scales, zeros, group)
+    t = _type(kind)
+    fi = torch.finfo(t)
+    small, large = (-14, 10) if kind == "f16" else (-60, 60)
+    for m in (1, 2, 3):
+        x = torch.randn(m, k, generator=gen, device=cuda)
+        wide = x * torch.exp2(torch.randint(small, large, (m, k), generator=gen, device=cuda).float())
+        per_group = x * torch.exp2(torch.randint(small, large, (m, 32), generator=gen, device=cuda).float()).repeat_interleave(32, 1)[:, :k]
+        zero = torch.zeros(m, k, device=cuda)
+        spikes = zero.clone()
+        spikes[:, ::97] = 3.0
+        ends = torch.full((m, k), 1.0, device=cuda) * (fi.max / 2 ** 8 if kind == "f16" else 2.0 ** 100)
+        tiny = x * fi.tiny * (1.0 if kind == "f16" else 2.0 ** 30)
+        for v in (wide, per_group, zero, spikes, ends, tiny):
+            v = v.to(t)
+            _check_product(w4.matvec(v, out_dtype=torch.float32), v, values, None, group)
+            if torch.isfinite(v.double() @ values.t()).all() and (v.double() @ values.t()).abs().max() < fi.max:
+                _check_product(w4.matvec(v), v, values, None, group)
+
+
+@pytest.mark.slow
+def test_more_than_2_to_32_codes(cuda, qrc):
+    """A matrix whose codes, packed words and scales lie beyond 2^32 bytes."""
+    import torch
+    k, group = 8192, 32
+    n = (1 << 32) // (k // 2) + 40                               # packed bytes pass 2^32, values 2^33
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    w = torch.empty(n, k, dtype=torch.float16, device=cuda)
+    for at in range(0, n, 1 << 16):
+        part = w[at:at + (1 << 16)]
+        part.copy_(torch.randn(part.shape, generator=gen, device=cuda))
+    w4 = qrc.quant_w4(w, group=group, symmetric=False)
+    assert w4.packed.numel() * 4 > 1 << 32
+    back = w4.dequant()
+    some = torch.tensor([0, 1, n // 2, n - 33, n - 2, n - 1], device=cuda)
+    codes, scales, zeros = _quant_reference(w[some], group, False)
+    assert torch.equal(w4.scales[:, some].double(), scales) and torch.equal(w4.zeros[:, some], zeros)
+    values = _values(codes, scales, zeros, group)
+    assert torch.equal(back[some], values.half())
+    for m in (1, 4):
+        x = torch.randn(m, k, generator=gen, device=cuda).half()
+        y = w4.matvec(x, out_dtype=torch.float32)
+        _check_product(y[:, some].contiguous(), x, values, None, group)
+        assert torch.isfinite(y).all()
