@@ -17,12 +17,12 @@ def stream_handle(stream, device: int):
     return (stream if isinstance(stream, int) else int(stream.cuda_stream)) or None
 
 
-def empty(shape, dtype, device, stream) -> torch.Tensor:
-    """torch.empty that belongs to the stream the call runs on, so that its
-    memory is not handed out again before the call is done."""
+def empty(shape, dtype, like: torch.Tensor, stream) -> torch.Tensor:
+    """New memory on `like`'s device that belongs to the stream the call runs
+    on, so that it is not handed out again before the call is done."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape) if dtype is like.dtype else like.new_empty(shape, dtype=dtype)
     if isinstance(stream, int):
-        stream = torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
+        stream = torch.cuda.ExternalStream(stream, device=like.device) if stream else torch.cuda.default_stream(like.device)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return torch.empty(shape, dtype=dtype, device=like.device)

@@ -105,10 +105,11 @@ class TensorList:
         h = ctypes.c_void_p()
         nat.check(self.lib, "qrc_list_create", self.lib.qrc_list_create(ctypes.byref(h), index, table, len(table)))
         self._h = h
-        self._work_bytes = int(self.lib.qrc_list_workspace(h))
+        self._work_floats = int(self.lib.qrc_list_workspace(h)) // 4
         # 1 when the outputs can be written without one changing another
         self._writable = self.lib.qrc_list_writable(table, len(table)) == 1
         self._torch_device = torch.device("cuda", index)
+        self._like = torch.empty(0, dtype=torch.float32, device=self._torch_device)
 
     def close(self) -> None:
         if getattr(self, "_h", None) is not None:
@@ -155,7 +156,7 @@ class TensorList:
         float64; a NaN element gives NaN.  The same bits on every call.
         Asynchronous."""
         code = self._order(ord)
-        out = empty((), torch.float32, self._torch_device, stream) if out is None else self._scalar(out, "out")
+        out = empty((), torch.float32, self._like, stream) if out is None else self._scalar(out, "out")
         work = self._work(stream)
         rc = self.lib.qrc_list_norm(self.handle, code, out.data_ptr(), None if work is None else work.data_ptr(),
                                     stream_handle(stream, self.device))
@@ -165,7 +166,7 @@ class TensorList:
 
     def _work(self, stream):
         """A workspace for one call; short lists need none."""
-        return empty(self._work_bytes, torch.uint8, self._torch_device, stream) if self._work_bytes else None
+        return empty(self._work_floats, torch.float32, self._like, stream) if self._work_floats else None
 
     def clip_norm(self, max_norm: float, ord: float = 2.0, norm: Optional[torch.Tensor] = None,
                   stream=None) -> torch.Tensor:
@@ -183,7 +184,7 @@ class TensorList:
         if norm is not None:
             given, result, work = self._scalar(norm, "norm").data_ptr(), norm, None
         else:
-            given, result, work = None, empty((), torch.float32, self._torch_device, stream), self._work(stream)
+            given, result, work = None, empty((), torch.float32, self._like, stream), self._work(stream)
         rc = self.lib.qrc_list_clip(self.handle, code, max_norm, given, result.data_ptr(),
                                     None if work is None else work.data_ptr(), stream_handle(stream, self.device))
         if rc:

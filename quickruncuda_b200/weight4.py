@@ -91,11 +91,11 @@ class Weight4:
         self._ref = ctypes.byref(self._w)
 
     @classmethod
-    def _new(cls, n: int, k: int, group: int, dtype, symmetric: bool, device, stream) -> "Weight4":
-        """A matrix with memory of its own, not filled yet."""
+    def _new(cls, n: int, k: int, group: int, symmetric: bool, like: torch.Tensor, stream) -> "Weight4":
+        """A matrix of `like`'s type with memory of its own, not filled yet."""
         w4, groups = cls.__new__(cls), (-(-k // group), n)
-        w4._set(empty(packed_shape(n, k), torch.int32, device, stream), empty(groups, dtype, device, stream),
-                None if symmetric else empty(groups, torch.uint8, device, stream), n, k, group)
+        w4._set(empty(packed_shape(n, k), torch.int32, like, stream), empty(groups, like.dtype, like, stream),
+                None if symmetric else empty(groups, torch.uint8, like, stream), n, k, group)
         return w4
 
     @classmethod
@@ -108,7 +108,7 @@ class Weight4:
             raise RuntimeError(f"Weight4: codes have to be 2-D, got {tuple(codes.shape)}")
         n, k = codes.shape
         ld = _pitch(codes, "codes")
-        w4 = cls(empty(packed_shape(n, k), torch.int32, codes.device, stream), scales, zeros, k, group)
+        w4 = cls(empty(packed_shape(n, k), torch.int32, codes, stream), scales, zeros, k, group)
         nat.check(w4.lib, "qrc_w4_pack",
                   w4.lib.qrc_w4_pack(w4._index, codes.data_ptr(), ld, w4._ref, stream_handle(stream, w4._index)))
         return w4
@@ -121,10 +121,11 @@ class Weight4:
             dtype = self.dtype if dtype is None else dtype
             if dtype not in _OUT_TYPES:
                 raise RuntimeError(f"Weight4: dequant needs dtype in {tuple(_OUT_TYPES)}, got {dtype}")
-            out = empty(self.shape, dtype, self.device, stream)
+            out, ld = empty(self.shape, dtype, self.scales, stream), self.shape[1]
         else:
             _check(out, "out", _OUT_TYPES if dtype is None else (dtype,), self.shape, self.device)
-        rc = self.lib.qrc_w4_dequant(self._index, self._ref, out.data_ptr(), _pitch(out, "out"), _OUT_TYPES[out.dtype],
+            dtype, ld = out.dtype, _pitch(out, "out")
+        rc = self.lib.qrc_w4_dequant(self._index, self._ref, out.data_ptr(), ld, _OUT_TYPES[dtype],
                                      stream_handle(stream, self._index))
         if rc:
             nat.check(self.lib, "qrc_w4_dequant", rc)
@@ -157,7 +158,7 @@ class Weight4:
             x2 = _as_rows(x, m, k, "x")
         ldx = k if x.is_contiguous() else _pitch(x2, "x")
         if out is None:
-            out, ldy = empty((*shape[:-1], n), kind, self.device, stream), n
+            out, ldy = empty((*shape[:-1], n), kind, x, stream), n
         else:
             _check(out, "out", (kind,), (*shape[:-1], n), self.device)
             ldy = _pitch(_as_rows(out, m, n, "out"), "out")
@@ -190,7 +191,7 @@ def quant_w4(w: torch.Tensor, group: int = 128, symmetric: bool = True, stream=N
         raise RuntimeError(f"Weight4: w has to be 2-D, got {tuple(w.shape)}")
     n, k = w.shape
     ld = _pitch(w, "w")
-    w4 = Weight4._new(n, k, _check_group(group), w.dtype, bool(symmetric), w.device, stream)
+    w4 = Weight4._new(n, k, _check_group(group), bool(symmetric), w, stream)
     rc = w4.lib.qrc_w4_quant(w4._index, w.data_ptr(), ld, int(bool(symmetric)), w4._ref, stream_handle(stream, w4._index))
     if rc:
         nat.check(w4.lib, "qrc_w4_quant", rc)
