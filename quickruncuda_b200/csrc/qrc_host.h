@@ -6,6 +6,7 @@
 #include <cstdint>
 #include <map>
 #include <mutex>
+#include <new>
 #include <utility>
 
 #define QRC_API extern "C" __attribute__((visibility("default")))
@@ -88,9 +89,13 @@ inline cudaError_t grant_smem(const void* kernel, size_t smem) {
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     std::lock_guard<std::mutex> lock(mu);
-    size_t& g = granted[{kernel, dev}];
-    if (smem <= g) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) g = smem;
-    return e;
+    try {
+        size_t& g = granted[{kernel, dev}];
+        if (smem <= g) return cudaSuccess;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e == cudaSuccess) g = smem;
+        return e;
+    } catch (const std::bad_alloc&) {
+        return cudaErrorMemoryAllocation;
+    }
 }

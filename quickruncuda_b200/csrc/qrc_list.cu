@@ -40,12 +40,12 @@ constexpr uint64_t kScaleBytes = 256 << 10;
 constexpr uint64_t kStreamBytes = 192ull << 20;
 constexpr uint32_t kFold = 1024;              // partial results that every block of the scale pass adds up itself
 constexpr int kMinChunkLog2 = 10, kMaxChunkLog2 = 15;
-// Up to this much input one cluster of blocks does everything in one launch: a
-// call takes 6 us of host time instead of 9.5 (norm) or 9.5 to 12 (clip), and
-// on the GPU about as long as two (256 KiB: norm 3.6 us, two launches 3.8).
-// Above it the eight SMs are what bounds it (1 MiB: 5.6 us, two launches 4.5).
+// Up to this much input one cluster of blocks does everything in one launch.
+// In a row of calls the host's launches count: 1 MiB of float32 takes 6.2 us
+// (norm) and 9.3 (clip), with two launches 9.0 and 10.4; at 2 MiB the eight
+// SMs are what bounds it, 7.4 and 13.9 against 8.9 and 10.5.
 constexpr int kCluster = 8, kSmallThreads = 256;
-constexpr uint64_t kSmallBytes = 512 << 10;
+constexpr uint64_t kSmallBytes = 1 << 20;
 constexpr int kKindShift = 56;                // n_kind: elements, input type << 56, output type << 60
 
 // One tensor: `n` elements at in and out.  cols == 0: dense; else rows of

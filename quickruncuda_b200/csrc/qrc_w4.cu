@@ -32,12 +32,12 @@ namespace {
 constexpr uint32_t kCodeMask = 0x00780078u;
 
 // What the kernels need of the two 16-bit types.  (bits & kCodeMask) | kOne is
-// the pair of values (kBias + code) * kUnit.
+// a constant plus the pair of values code * kUnit.
 template <class T> struct Half;
 template <> struct Half<__nv_bfloat16> {
     using Pair = __nv_bfloat162;
     static constexpr uint32_t kOne = 0x41804180u;
-    static constexpr float kBias = 16.0f, kUnit = 1.0f;
+    static constexpr float kUnit = 1.0f;
     static constexpr float kMax = 3.3895313892515355e38f, kLeastScale = 0x1p-100f, kMostScale = 0x1p100f;
     // Within four float steps of the middle between two values of the type.
     static __device__ __forceinline__ bool near_border(float f) { return (__float_as_uint(f) & 0xffffu) - 0x7ffcu <= 8u; }
@@ -67,7 +67,7 @@ template <> struct Half<__nv_bfloat16> {
 template <> struct Half<__half> {
     using Pair = __half2;
     static constexpr uint32_t kOne = 0u;
-    static constexpr float kBias = 0.0f, kUnit = 0x1p-21f;
+    static constexpr float kUnit = 0x1p-21f;
     static constexpr float kMax = 65504.0f, kLeastScale = 0x1p-13f, kMostScale = 65504.0f;
     static __device__ __forceinline__ bool near_border(float f) { return (__float_as_uint(f) & 0x1fffu) - 0x0ffcu <= 8u; }
     static __device__ __forceinline__ uint64_t widen(uint32_t p) {
@@ -103,7 +103,7 @@ template <class T> __device__ __forceinline__ uint32_t to_bits(T x) { return rei
 
 __device__ __forceinline__ uint32_t rotate_right(uint32_t w, int by) { return __funnelshift_r(w, w, by); }
 
-// Columns 2*i and 2*i + 1 of a word as a pair of T: (kBias + code) * kUnit.
+// Columns 2*i and 2*i + 1 of a word as a pair of T: a constant plus code * kUnit.
 template <class T> __device__ __forceinline__ uint32_t code_pair(uint32_t word, int i) {
     return (rotate_right(word, 4 * i) & kCodeMask) | Half<T>::kOne;
 }
@@ -116,11 +116,6 @@ __device__ __forceinline__ int code_shift(int e) { return (3 + (e >> 1) * 4 + (e
 
 __device__ __forceinline__ uint32_t place_code(uint32_t code, int e) {
     return __funnelshift_l(code, code, code_shift(e));
-}
-
-// Word `i` of row `row`, tile column `tile`, of a matrix `tiles` tiles wide.
-__device__ __forceinline__ uint64_t word_at(uint64_t row, uint64_t tile, uint64_t tiles, uint32_t i) {
-    return ((row >> 4) * tiles + tile) * 256 + (row & 15) * 16 + i;
 }
 
 // Blocks of four warps, a warp per 4 or 8 rows and 256 columns.  A 16384 x 8192
