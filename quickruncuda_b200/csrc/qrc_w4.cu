@@ -14,7 +14,10 @@
 // bit 3 + 4*(e / 2) + 16*(e % 2), modulo 32: a rotation by 0, 4, 8 or 12 and
 // one mask bring two neighbouring columns to bits 3..6 of both halves.  There
 // they are the upper mantissa bits of a bfloat16 (16 + code with the exponent
-// of 16) or an fp16 subnormal (code * 2^-21).  Read as bytes, the same word
+// of 16) or lower ones of an fp16 (1024 + 8 * code with the exponent of 1024).
+// Left alone they would be fp16 subnormals, code * 2^-21, at no cost; but the
+// matrix instruction adds products of subnormals to 2^-19 of their sum only.
+// Read as bytes, the same word
 // holds four codes times 8 under the mask 0x78787878, and the other four
 // after a rotation by 4.
 #define QRC_NO_PLUGIN_ABI
@@ -43,10 +46,7 @@ template <> struct Half<__nv_bfloat16> {
     static __device__ __forceinline__ bool near_border(float f) { return (__float_as_uint(f) & 0xffffu) - 0x7ffcu <= 8u; }
     // A pair as two floats.
     static __device__ __forceinline__ uint64_t widen(uint32_t p) { return (uint64_t)(p & 0xffff0000u) << 32 | p << 16; }
-    // (bits & kCodeMask) | kWide is a constant plus code / kWideUnit, with room
-    // to subtract a zero's and multiply by scale * kWideUnit.
-    static constexpr uint32_t kWide = 0x41804180u;
-    static constexpr float kWideUnit = 1.0f, kLeastWide = kLeastScale;
+    static constexpr float kLeastWide = kLeastScale;      // scale / kUnit is exact from here on
     static __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
         const Pair r = __hsub2(reinterpret_cast<Pair&>(a), reinterpret_cast<Pair&>(b));
         return reinterpret_cast<const uint32_t&>(r);
@@ -66,16 +66,15 @@ template <> struct Half<__nv_bfloat16> {
 };
 template <> struct Half<__half> {
     using Pair = __half2;
-    static constexpr uint32_t kOne = 0u;
-    static constexpr float kUnit = 0x1p-21f;
+    static constexpr uint32_t kOne = 0x64006400u;
+    static constexpr float kUnit = 8.0f;
     static constexpr float kMax = 65504.0f, kLeastScale = 0x1p-13f, kMostScale = 65504.0f;
     static __device__ __forceinline__ bool near_border(float f) { return (__float_as_uint(f) & 0x1fffu) - 0x0ffcu <= 8u; }
     static __device__ __forceinline__ uint64_t widen(uint32_t p) {
         const float2 f = __half22float2(reinterpret_cast<__half2&>(p));
         return (uint64_t)__float_as_uint(f.y) << 32 | __float_as_uint(f.x);
     }
-    static constexpr uint32_t kWide = 0x64006400u;
-    static constexpr float kWideUnit = 0.125f, kLeastWide = 0x1p-11f;     // an eighth is exact
+    static constexpr float kLeastWide = 0x1p-11f;
     static __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
         const Pair r = __hsub2(reinterpret_cast<Pair&>(a), reinterpret_cast<Pair&>(b));
         return reinterpret_cast<const uint32_t&>(r);
@@ -548,11 +547,11 @@ qrc_k_w4_dequant(const uint32_t* packed, const uint16_t* scales, const uint8_t* 
             uint32_t v[WORDS];
             const float s = Half<T>::to_float(from_bits<T>(scale[r]));
             if (std::is_same<T, TO>::value && s >= Half<T>::kLeastWide && s <= Half<T>::kMax / 16) {
-                const uint32_t m = to_bits(Half<T>::round(s * Half<T>::kWideUnit)) * 0x10001u;
-                const uint32_t z = zero[r] * 0x80008u | Half<T>::kWide;
+                const uint32_t m = to_bits(Half<T>::round(s * (1.0f / Half<T>::kUnit))) * 0x10001u;
+                const uint32_t z = zero[r] * 0x80008u | Half<T>::kOne;
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    v[i] = Half<T>::mul2(Half<T>::sub2((rotate_right(word[r], 4 * i) & kCodeMask) | Half<T>::kWide, z), m);
+                    v[i] = Half<T>::mul2(Half<T>::sub2(code_pair<T>(word[r], i), z), m);
             } else {
                 __align__(16) TO f[8];
 #pragma unroll

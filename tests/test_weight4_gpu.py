@@ -231,6 +231,20 @@ def test_matvec_of_views(cuda, qrc, kind):
         w4.matvec(buf[:, :2 * k].view(12, 2, k), bias=bias)
 
 
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_matvec_adds_in_float(cuda, qrc, kind):
+    """Few columns leave little room: the tolerance is some ten float steps of
+    the terms' sum, and sums of products kept to fewer bits than float's show."""
+    import torch
+    for k in (2, 3, 5, 8, 16, 31):
+        codes, scales, zeros, gen = _case(cuda, 496, k, kind, 128, False, seed=k)
+        w4 = qrc.Weight4.from_codes(codes, scales, zeros, group=128)
+        values = _values(codes, scales, zeros, 128)
+        for m in (1, 2, 3, 9, 17, 70):
+            x = torch.randn(m, k, generator=gen, device=cuda).to(_type(kind))
+            _check_product(w4.matvec(x, out_dtype=torch.float32), x, values, None, 128)
+
+
 def test_matvec_edges(cuda, qrc):
     import torch
     codes, scales, zeros, gen = _case(cuda, 40, 300, "bf16", 128, True)
