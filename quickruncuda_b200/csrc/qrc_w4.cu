@@ -265,10 +265,14 @@ qrc_k_w4_quant(const uint16_t* w, uint64_t ld, uint64_t n, uint64_t k, uint32_t*
         const uint64_t tile = k0 >> 7;
         uint32_t* const to = packed + ((first >> 4) * tiles + tile) * 256 + (first & 15) * 16 + (lane & 3) * 4 + ((lane >> 2) & 3);
         uint4 v[ROWS];
+        const uint16_t* const p = w + first * ld + k0;
+        if (VEC && first + ROWS <= n && k0 - lane * 8 + 256 <= k) {         // all of the window is there
 #pragma unroll
-        for (int r = 0; r < ROWS; r++) {
-            const uint64_t row = first + r;
-            v[r] = row < n && have ? load_eight<VEC>(w + row * ld + k0, have, w, end) : make_uint4(0, 0, 0, 0);
+            for (int r = 0; r < ROWS; r++) v[r] = *reinterpret_cast<const uint4*>(p + r * ld);
+        } else {
+#pragma unroll
+            for (int r = 0; r < ROWS; r++)
+                v[r] = first + r < n && have ? load_eight<VEC>(p + r * ld, have, w, end) : make_uint4(0, 0, 0, 0);
         }
         auto as_pair = [](uint32_t x) { return reinterpret_cast<Pair&>(x); };
         auto as_bits = [](Pair x) { return reinterpret_cast<uint32_t&>(x); };
@@ -326,7 +330,11 @@ qrc_k_w4_quant(const uint16_t* w, uint64_t ld, uint64_t n, uint64_t k, uint32_t*
             }
         }
 #pragma unroll
-        for (int r = 0; r < ROWS; r++) usual = usual && (s[r] == 0.0f || (s[r] >= Half<T>::kLeastScale && s[r] <= Half<T>::kMostScale));
+        for (int r = 0; r < ROWS; r++) {
+            // 0, or from kLeastScale to kMostScale; NaN is neither
+            const uint32_t bits = __float_as_uint(s[r]), least = __float_as_uint(Half<T>::kLeastScale);
+            usual = usual && (bits == 0 || bits - least <= __float_as_uint(Half<T>::kMostScale) - least);
+        }
         if (__any_sync(0xffffffffu, !usual)) {
 #pragma unroll 1
             for (int r = 0; r < ROWS; r++) {
