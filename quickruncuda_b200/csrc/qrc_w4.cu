@@ -117,10 +117,12 @@ __device__ __forceinline__ uint32_t place_code(uint32_t code, int e) {
     return __funnelshift_l(code, code, code_shift(e));
 }
 
-// Blocks of four warps, a warp per 4 or 8 rows and 256 columns.  A 16384 x 8192
-// matrix of bf16 quantizes in 70 us with eight rows loaded at a time, 77 with
-// four; with zeros (more registers) or unaligned rows (more instructions per
-// load) it is the other way round: fp16 with zeros 114 and 105 us.
+// Blocks of four warps, a warp per 4 or 8 rows and 256 columns.  With eight
+// rows loaded at a time a 16384 x 8192 matrix of bf16 quantizes in 60 us (the
+// memory's time is 51; with four rows, measured before whole windows went
+// without guards, 77 against 70).  With zeros, which take more registers, four
+// rows are faster (fp16, groups of 32: 89 against 97 us), and so they are for
+// unaligned rows.
 constexpr int kWindowWarps = 4, kWindowThreads = 32 * kWindowWarps, kDequantRows = 8;
 template <bool SYMMETRIC, bool VEC> constexpr int kQuantRows = SYMMETRIC && VEC ? 8 : 4;
 
@@ -299,7 +301,8 @@ qrc_k_w4_quant(const uint16_t* w, uint64_t ld, uint64_t n, uint64_t k, uint32_t*
         constexpr int COUNT = SYMMETRIC ? ROWS / 2 : ROWS;
         bool usual = true;
         uint32_t scale[ROWS];
-        float s[ROWS], zero[ROWS];
+        float s[ROWS];
+        uint32_t zero[ROWS];
 #pragma unroll
         for (int i = 0; i < COUNT; i++) {
 #pragma unroll
@@ -314,7 +317,7 @@ qrc_k_w4_quant(const uint16_t* w, uint64_t ld, uint64_t n, uint64_t k, uint32_t*
                 s[2 * i + 1] = Half<T>::to_float(b);
                 scale[2 * i] = to_bits(a);
                 scale[2 * i + 1] = to_bits(b);
-                zero[2 * i] = zero[2 * i + 1] = 8.0f;
+                zero[2 * i] = zero[2 * i + 1] = 8;
             } else {
                 // The difference, exact as sum and error; its fifteenth in
                 // float decides unless it is within four steps of a border.
@@ -358,10 +361,8 @@ qrc_k_w4_quant(const uint16_t* w, uint64_t ld, uint64_t n, uint64_t k, uint32_t*
             constexpr float kRound = 12582912.0f;               // 1.5 * 2^23: adding it rounds to whole numbers
             if (!SYMMETRIC) {
                 const float least = Half<T>::to_float(from_bits<T>(most[r] >> 16));      // -minimum
-                float z0, z1;
                 const uint64_t q = add2(divide2(pair_of(least, 0.0f), r2, minus_s), pair_of(kRound, kRound));
-                asm("mov.b64 {%0, %1}, %2;" : "=f"(z0), "=f"(z1) : "l"(q));
-                zero[r] = z0 - kRound;
+                zero[r] = (uint32_t)q & 0xffffu;
             }
             const uint32_t x[4] = {v[r].x, v[r].y, v[r].z, v[r].w};
             uint32_t p[4];
@@ -369,17 +370,11 @@ qrc_k_w4_quant(const uint16_t* w, uint64_t ld, uint64_t n, uint64_t k, uint32_t*
             for (int i = 0; i < 4; i++) {
                 uint64_t q = divide2(Half<T>::widen(x[i]), r2, minus_s);
                 uint32_t c0, c1;
-                if (SYMMETRIC) {
-                    q = add2(q, pair_of(kRound + 8.0f, kRound + 8.0f));
-                    asm("mov.b64 {%0, %1}, %2;" : "=r"(c0), "=r"(c1) : "l"(q));
-                } else {
-                    float f0, f1;
-                    q = add2(add2(q, pair_of(kRound, kRound)), pair_of(zero[r], zero[r]));
-                    asm("mov.b64 {%0, %1}, %2;" : "=f"(f0), "=f"(f1) : "l"(q));
-                    c0 = __float_as_uint(fminf(f0, kRound + 15.0f));
-                    c1 = __float_as_uint(fminf(f1, kRound + 15.0f));
-                }
-                p[i] = __byte_perm(c0, c1, 0x5410);             // the codes are the last bits
+                constexpr float kAdd = SYMMETRIC ? kRound + 8.0f : kRound;
+                q = add2(q, pair_of(kAdd, kAdd));
+                asm("mov.b64 {%0, %1}, %2;" : "=r"(c0), "=r"(c1) : "l"(q));
+                p[i] = __byte_perm(c0, c1, 0x5410);                 // whole numbers in the last 16 bits
+                if (!SYMMETRIC) p[i] = __viaddmin_s16x2(p[i], __byte_perm(zero[r], 0, 0x1010), 0x000f000fu);
             }
             const uint32_t word = p[0] + p[1] * 16u + p[2] * 256u + p[3] * 4096u;
             if (tile < tiles) to[r * 16] = __funnelshift_l(word, word, 3);
@@ -389,8 +384,7 @@ qrc_k_w4_quant(const uint16_t* w, uint64_t ld, uint64_t n, uint64_t k, uint32_t*
         if (k0 - member * 8 < k) {
 #pragma unroll
             for (int r0 = 0; r0 < ROWS; r0 += LANES) {
-                uint32_t mine = 0;
-                float z = 0.0f;
+                uint32_t mine = 0, z = 0;
 #pragma unroll
                 for (int r = r0; r < r0 + LANES && r < ROWS; r++) {
                     if (member == r - r0) { mine = scale[r]; z = zero[r]; }
