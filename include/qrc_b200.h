@@ -400,7 +400,7 @@ int qrc_w4_dequant(int device, const qrc_w4* w, void* d_out, uint64_t ld, int ou
  * are of w->type, d_y of y_type: w->type or QRC_F32.  Products and sums are
  * formed in float, per group before its scale (so |x| * 15 * group has to
  * stay in float's range), in an order that depends on the sizes alone; the
- * result is rounded once.  With one or two rows x enters as whole numbers of
+ * result is rounded once.  With up to five rows x may enter as whole numbers of
  * 2^-21 of the power of two at its group's largest magnitude (of 2^-126 at
  * least).  Made for a few rows (a decode step); any m >= 0 works.  An infinite or NaN activation gives NaN.  If a bounded wait inside
  * the kernel gives up (about 1 s), the results are NaN.  Asynchronous. */

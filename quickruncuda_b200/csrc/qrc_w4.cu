@@ -660,8 +660,8 @@ struct Shape {
 //   summed in float; the scale of a group (128 / SUB columns, or a multiple of
 //   128 with SUB = 1) multiplies the group's sum.  Eleven instructions per
 //   eight codes.
-// * DIGITS, for one or two rows of activations: codes as bytes, three
-//   instructions per eight.  x of a group is written as whole numbers of
+// * DIGITS, for one or two rows of activations (up to five where it pays):
+//   codes as bytes, three instructions per eight.  x of a group is written as whole numbers of
 //   2^(e-21), e the exponent of its largest magnitude, and those as three
 //   signed bytes (hi * 2^16 + mid * 2^8 + lo), a column of the matrix
 //   instruction each.  A bfloat16 down to 2^-14 of the group's largest is
@@ -1089,10 +1089,14 @@ int launch_shape(const qrc_w4& w, const T* x, uint64_t ldx, uint64_t m, const T*
         QRC_CK(launch_overlapped(kernel, grid, S::W * 32, smem, s, cluster, a, x, ldx, m, bias, y, ldy, y_float, x_vec, chunk_tiles, cluster));
         return QRC_OK;
     };
-    switch (sub) {
-        case 4: return w.d_zeros ? go(qrc_k_w4_matvec<T, S, 4, true>) : go(qrc_k_w4_matvec<T, S, 4, false>);
-        case 2: return w.d_zeros ? go(qrc_k_w4_matvec<T, S, 2, true>) : go(qrc_k_w4_matvec<T, S, 2, false>);
-        default: return w.d_zeros ? go(qrc_k_w4_matvec<T, S, 1, true>) : go(qrc_k_w4_matvec<T, S, 1, false>);
+    if constexpr (S::DIGITS && S::NT > 1) {                     // only taken with large groups
+        return w.d_zeros ? go(qrc_k_w4_matvec<T, S, 1, true>) : go(qrc_k_w4_matvec<T, S, 1, false>);
+    } else {
+        switch (sub) {
+            case 4: return w.d_zeros ? go(qrc_k_w4_matvec<T, S, 4, true>) : go(qrc_k_w4_matvec<T, S, 4, false>);
+            case 2: return w.d_zeros ? go(qrc_k_w4_matvec<T, S, 2, true>) : go(qrc_k_w4_matvec<T, S, 2, false>);
+            default: return w.d_zeros ? go(qrc_k_w4_matvec<T, S, 1, true>) : go(qrc_k_w4_matvec<T, S, 1, false>);
+        }
     }
 }
 
@@ -1107,7 +1111,13 @@ int launch_matvec(const qrc_w4& w, const void* d_x, uint64_t m, uint64_t ldx, co
         const T* x = static_cast<const T*>(d_x) + m0 * ldx;
         void* y = static_cast<char*>(d_y) + m0 * ldy * (y_float ? 4 : 2);
         auto go = [&](auto shape) { return launch_shape<T, decltype(shape)>(w, x, ldx, rows, bias, y, ldy, y_float, sms, s); };
-        const int rc = rows <= 2 ? go(Shape<true, 1, 16, 4, 2>())
+        // Three to five rows as bytes take six to fifteen columns, and every
+        // block turns the rows into bytes anew: worth it with a scale per 128
+        // columns or more and enough rows of weights per block.  65536 x 8192,
+        // 3, 4, 5 rows: 67, 76, 79 us, in 16 bits 85; 16384 x 8192: 23, 25, 27
+        // and 25.
+        const bool bytes = rows <= 5 && w.group >= 128 && (w.n + 15) / 16 >= 3 * (rows - 1) * sms;
+        const int rc = rows <= 2 ? go(Shape<true, 1, 16, 4, 2>()) : bytes ? go(Shape<true, 2, 16, 4, 2>())
                        : rows <= 8 ? go(Shape<false, 1, 16, 4, 2>())
                        : rows <= 16 ? go(Shape<false, 2, 12, 4, 2>()) : go(Shape<false, 4, 8, 4, 2>());
         if (rc != QRC_OK) return rc;

@@ -245,6 +245,27 @@ def test_matvec_adds_in_float(cuda, qrc, kind):
             _check_product(w4.matvec(x, out_dtype=torch.float32), x, values, None, 128)
 
 
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_matvec_many_rows_of_weights(cuda, qrc, kind, symmetric):
+    """Enough rows of weights that a few activations go through bytes, several
+    passes per block, with and without paired blocks."""
+    import torch
+    for n, k, group in ((30_011, 520, 128), (45_000, 129, 256), (2400, 3001, 128)):
+        codes, scales, zeros, gen = _case(cuda, n, k, kind, group, symmetric, seed=n)
+        w4 = qrc.Weight4.from_codes(codes, scales, zeros, group=group)
+        values = _values(codes, scales, zeros, group)
+        for m in (1, 2, 3, 4, 5, 6):
+            x = torch.randn(m, k, generator=gen, device=cuda).to(_type(kind))
+            bias = torch.randn(n, generator=gen, device=cuda).to(_type(kind))
+            _check_product(w4.matvec(x, bias=bias, out_dtype=torch.float32), x, values, bias, group)
+            x[m - 1, k // 2] = math.inf
+            y = w4.matvec(x)
+            assert not torch.isfinite(y[m - 1]).any()
+            if m > 1:
+                _check_product(y[:m - 1], x[:m - 1], values, None, group)
+
+
 def test_matvec_edges(cuda, qrc):
     import torch
     codes, scales, zeros, gen = _case(cuda, 40, 300, "bf16", 128, True)
