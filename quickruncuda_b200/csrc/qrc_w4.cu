@@ -617,6 +617,12 @@ __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// The warp's wait for a barrier's phase, bounded; all lanes agree on whether it
+// came, so that none goes on without the others.
+__device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, qrc::mbar_wait_bounded(bar, parity));
+}
+
 __device__ __forceinline__ void mma_bytes(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
@@ -885,7 +891,7 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias,
                 __syncthreads();
                 if (!DIGITS) {
                     if (chunk + 1 < chunks) stage_half(chunk + 1, buffer ^ 1);
-                    if (!qrc::mbar_wait_bounded(x_bars + 8 * buffer, (x_parity >> buffer) & 1)) failed = true;
+                    if (!wait_all(x_bars + 8 * buffer, (x_parity >> buffer) & 1)) failed = true;
                     x_parity ^= 1u << buffer;
                 }
                 staged = true;
@@ -897,7 +903,7 @@ qrc_k_w4_matvec(const W4 w, const T* x, uint64_t ldx, uint64_t m, const T* bias,
 #pragma unroll
                 for (int i = 0; i < kUnits; i++) now[i] = scale[i] | (ZEROS ? zero[i] : 8u) << 19;
                 if (at + BT < hi) load_scales(tile_of(chunk) + at + BT);
-                if (failed || !qrc::mbar_wait_bounded(bars + 8 * slot, (parity >> slot) & 1)) { failed = true; break; }
+                if (failed || !wait_all(bars + 8 * slot, (parity >> slot) & 1)) { failed = true; break; }
                 parity ^= 1u << slot;
                 filled &= ~(1u << slot);
                 const uint32_t q = ring_at + slot * S::kSlot + lane * 16;
