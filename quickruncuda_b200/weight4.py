@@ -146,6 +146,8 @@ class Weight4:
             raise RuntimeError(f"Weight4: x has shape {tuple(shape)}, needs [..., {k}]")
         if bias is not None:
             _check(bias, "bias", (self.dtype,), (n,), self.device)
+            if bias.requires_grad and torch.is_grad_enabled():
+                raise RuntimeError("Weight4: matvec has no backward pass; call it under torch.no_grad() or with bias.detach()")
             if n > 1 and bias.stride(0) != 1:
                 raise RuntimeError("Weight4: bias has to be contiguous")
         kind = out_dtype if out_dtype is not None else out.dtype if out is not None else self.dtype

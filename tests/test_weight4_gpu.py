@@ -379,6 +379,17 @@ def test_backward_is_refused(cuda, qrc):
         assert torch.equal(w4.matvec(x), w4.matvec(x.detach()))
 
 
+def test_backward_through_the_bias_is_refused(cuda, qrc):
+    import torch
+    w4 = qrc.quant_w4(torch.randn(16, 64, device=cuda).half())
+    x = torch.randn(2, 64, device=cuda).half()
+    bias = torch.randn(16, device=cuda).half().requires_grad_()
+    with pytest.raises(RuntimeError, match="backward"):
+        w4.matvec(x, bias=bias)
+    with torch.no_grad():
+        assert torch.equal(w4.matvec(x, bias=bias), w4.matvec(x, bias=bias.detach()))
+
+
 @pytest.mark.parametrize("kind", ["bf16", "f16"])
 def test_matvec_activations_of_any_size(cuda, qrc, kind):
     """One and two rows go through whole numbers scaled per group: ranges that
