@@ -83,12 +83,18 @@ class Weight4:
 
     def _set(self, packed, scales, zeros, n: int, k: int, group: int) -> None:
         self.lib = nat.load()
-        self.packed, self.scales, self.zeros = packed, scales, zeros
+        self._packed, self._scales, self._zeros = packed, scales, zeros
         self.shape, self.group, self.dtype, self.device = (n, k), group, scales.dtype, packed.device
         self._index = packed.device.index
         self._w = nat.W4(packed.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(), n, k, group,
                          _TYPES[scales.dtype])
         self._ref = ctypes.byref(self._w)
+
+    # The calls read these tensors' memory where the constructor found it:
+    # other tensors need another Weight4.
+    packed = property(lambda self: self._packed)
+    scales = property(lambda self: self._scales)
+    zeros = property(lambda self: self._zeros)
 
     @classmethod
     def _new(cls, n: int, k: int, group: int, symmetric: bool, like: torch.Tensor, stream) -> "Weight4":

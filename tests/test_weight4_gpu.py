@@ -379,6 +379,19 @@ def test_backward_is_refused(cuda, qrc):
         assert torch.equal(w4.matvec(x), w4.matvec(x.detach()))
 
 
+def test_tensors_of_a_matrix_are_not_replaced(cuda, qrc):
+    """The product would go on reading the old ones."""
+    import torch
+    w4 = qrc.quant_w4(torch.randn(16, 64, device=cuda).half(), symmetric=False)
+    for name in ("packed", "scales", "zeros"):
+        with pytest.raises(AttributeError):
+            setattr(w4, name, getattr(w4, name).clone())
+    x = torch.ones(1, 64, dtype=torch.float16, device=cuda)
+    y = w4.matvec(x, out_dtype=torch.float32)
+    w4.scales.mul_(2)                                               # in place: seen by the next call
+    assert torch.equal(w4.matvec(x, out_dtype=torch.float32), 2 * y)
+
+
 def test_backward_through_the_bias_is_refused(cuda, qrc):
     import torch
     w4 = qrc.quant_w4(torch.randn(16, 64, device=cuda).half())
