@@ -6,8 +6,10 @@ gradient clipping of a training step (qrc_list_* of include/qrc_b200.h).
 
 A `TensorList` is a plan: it is made once, keeps the tensors alive and can be
 used from any stream, thread or captured graph.  It holds the tensors it was
-given: gradients that a later step allocates anew need a new list (with
-`zero_grad(set_to_none=False)` they stay where they are).
+given, at the memory they had then: gradients that a later step allocates anew
+or that are given other memory (`.data = ...`, `set_`) need a new list (with
+`zero_grad(set_to_none=False)` they stay where they are).  A storage must not
+be resized while a list holds it.
 """
 from __future__ import annotations
 
@@ -68,6 +70,9 @@ def _describe(tensors: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tens
                 raise RuntimeError(f"TensorList needs dtypes in {tuple(_TYPES)}, got {t.dtype}")
             if t.layout != torch.strided:
                 raise RuntimeError(f"TensorList needs strided tensors, got {t.layout}")
+            if t.is_neg():
+                raise RuntimeError("TensorList needs tensors whose sign is in their memory, got a negated view; "
+                                   "call resolve_neg() on it")
             if device is None:
                 device = t.device
             elif t.device != device:
@@ -94,8 +99,12 @@ class TensorList:
     def __init__(self, tensors: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]] = None,
                  device: Optional[int] = None):
         self.lib = nat.load()
-        self.tensors = list(tensors)
-        self.out = self.tensors if out is None else list(out)
+        self.tensors = tuple(tensors)
+        self.out = self.tensors if out is None else tuple(out)
+        # The memory itself is kept too: it stays when a tensor is given other
+        # memory (`.data = ...`, `set_`).
+        self._memory = [t.untyped_storage() for t in (*self.tensors, *(() if out is None else self.out))
+                        if t.layout == torch.strided]
         table, index = _describe(self.tensors, None if out is None else self.out)
         if index is None:
             index = torch.cuda.current_device() if device is None else int(device)

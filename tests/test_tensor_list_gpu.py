@@ -292,6 +292,26 @@ def test_two_streams_and_graphs_share_a_list(cuda, qrc):
     assert abs(float(n) - want[2.0]) <= 5 * U * want[2.0]
 
 
+def test_memory_is_kept_when_a_tensor_is_given_another(cuda, qrc):
+    import torch
+    a = torch.full((1 << 20,), 2.0, device=cuda)
+    at = a.data_ptr()
+    with qrc.TensorList([a]) as grads:
+        a.data = torch.full((1 << 20,), 3.0, device=cuda)
+        other = [torch.empty(1 << 20, device=cuda) for _ in range(4)]
+        assert all(t.data_ptr() != at for t in other)               # nobody else was given that memory
+        assert grads.norm().item() == 2.0 * 2 ** 10                 # sqrt(2^20 * 4), exact
+        assert a.min().item() == 3.0
+
+
+def test_negated_views_are_refused(cuda, qrc):
+    import torch
+    a = torch.ones(8, device=cuda)
+    for args in (([torch._neg_view(a)],), ([a], [torch._neg_view(torch.ones(8, device=cuda))])):
+        with pytest.raises(RuntimeError, match="resolve_neg"):
+            qrc.TensorList(*args)
+
+
 def test_follows_the_stream_order(cuda, qrc):
     """Overlapped launches still wait for what the stream did before."""
     import torch
